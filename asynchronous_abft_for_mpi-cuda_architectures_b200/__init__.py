@@ -40,7 +40,7 @@ def __getattr__(name):
     if name in ("OnlineSession",):
         from .session import OnlineSession
         return OnlineSession
-    if name in ("kernels", "session", "distributed"):
+    if name in ("kernels", "products", "session", "distributed"):
         import importlib
         return importlib.import_module(f".{name}", __name__)
     raise AttributeError(name)

@@ -91,6 +91,7 @@ _I64 = ctypes.c_int64
 _U64 = ctypes.c_uint64
 _D = ctypes.c_double
 _F = ctypes.c_float
+_Z = ctypes.c_size_t
 _IP = ctypes.POINTER(ctypes.c_int)
 _DP = ctypes.POINTER(ctypes.c_double)
 
@@ -128,6 +129,16 @@ SIGNATURES = {
     "abft_inject_add": (_I, [_P, _I64, _I, _I, _F, _P]),
     "abft_inject_bitflip": (_I, [_P, _I64, _I, _I, _I, _P]),
     "abft_sgemm": (_I, [_P, _P, _I, _P, _I, _P, _I, _I, _I, _I]),
+    "abft_quantize_rows": (_I, [_P, _I64, _I, _I, _I, _P, _I64, _P, _P, _P, _P]),
+    "abft_column_checksum": (_I, [_P, _I64, _I, _I, _P, _P]),
+    "abft_int8_matmul_ws_bytes": (_Z, [_P, _I64, _P, _I64, _I, _I, _I]),
+    "abft_int8_matmul": (_I, [_P, _I64, _P, _P, _I64, _P, _I, _I, _I, _P, _I64, _I, _P, _P, _P, _Z, _P]),
+    "abft_gated_ffn_ws_bytes": (_Z, [_P, _I64, _P, _I64, _P, _I64, _I, _I, _I]),
+    "abft_gated_ffn": (_I, [_P, _I64, _P, _I64, _P, _I64, _I, _I, _I, _I, _I, _P, _I64, _P, _I64, _P, _I64, _P, _Z,
+                            _P]),
+    "abft_gated_ffn_backward_ws_bytes": (_Z, [_P, _I64, _P, _I64, _P, _I64, _I, _I, _I]),
+    "abft_gated_ffn_backward": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I, _I, _I, _I, _I,
+                                     _P, _I64, _P, _I64, _P, _I64, _P, _Z, _P]),
     "abft_session_create": (_I, [ctypes.POINTER(SessionCfg), ctypes.POINTER(_P)]),
     "abft_session_destroy": (_I, [_P]),
     "abft_session_ws": (_P, [_P]),

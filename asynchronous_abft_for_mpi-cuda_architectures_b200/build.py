@@ -26,7 +26,7 @@ CUDA_LIB = os.path.join(CUDA_HOME, "lib64")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 HOST_FLAGS = "-fPIC,-ffp-contract=off,-O2"
 
-LIB_CU = ["abft_kernels.cu", "abft_capi.cu", "abft_pipeline.cu"]
+LIB_CU = ["abft_kernels.cu", "abft_capi.cu", "abft_pipeline.cu", "abft_products.cu"]
 LIB_CPP = ["abft_host.cpp", "abft_report.cpp"]
 DRIVER_SRC = ["abft_gemm_main.cpp", "abft_comm.cpp"]
 

@@ -40,6 +40,17 @@ extern "C" {
 #define ABFT_SEED_REFERENCE 0 /* injection draws of the reference (per rank, per iteration) */
 #define ABFT_SEED_TILE 1      /* abft_injection_plan_tile with seed = base_seed + iteration  */
 
+#define ABFT_TYPE_F32 0  /* element types of the language-model products */
+#define ABFT_TYPE_F16 1
+#define ABFT_TYPE_BF16 2
+
+#define ABFT_ACT_SILU 0      /* activations of the gated feed-forward block */
+#define ABFT_ACT_GELU 1      /* g * Phi(g)                                  */
+#define ABFT_ACT_GELU_TANH 2 /* its tanh approximation                      */
+
+#define ABFT_INT8_MAX_K 131071      /* 128 * 128 * K fits a 32-bit sum      */
+#define ABFT_INT8_MAX_ROWS 16777216 /* 127 * N fits a 32-bit checksum       */
+
 #define ABFT_CORRECT_INLOOP 0 /* correct inside the loop (reference behaviour) */
 #define ABFT_CORRECT_DRAIN 1  /* locate in the loop, correct after it          */
 
@@ -234,6 +245,78 @@ int abft_inject_bitflip(float* dC, int64_t ldc, int row, int col, int bit, void*
  * (gemm_cublas, kernels/gemm_cublas.cuh:7-22): C = A * B, A M x K, B K x N. */
 int abft_sgemm(void* cublas_handle, const float* dA, int lda, const float* dB, int ldb, float* dC, int ldc, int M,
                int N, int K);
+
+/* ------------------------------------------------------------------------
+ * Products of language models (no counterpart in the reference, whose only
+ * product is the SGEMM above). Enqueue only, on the caller's stream; nothing
+ * is allocated and no state is kept between calls, so calls on different
+ * streams are independent as long as their outputs and workspaces are. The
+ * current device must be the stream's. Matrices are row-major with a pitch in
+ * elements; a weight is N x K (one row per output channel). Element types are
+ * ABFT_TYPE_*. T may be 0. Inputs and outputs must not overlap.
+ *
+ * Workspaces: each *_ws_bytes function takes the inputs of its call and says
+ * how many bytes of 16-byte aligned device memory that call needs as dWork
+ * (often 0, then dWork may be NULL). It is scratch: free for other use once
+ * the call's work has finished, and not shared by calls that may overlap.
+ * Operands whose base or pitch is not a multiple of 16 bytes are supported;
+ * they are copied into the workspace first.
+ * ---------------------------------------------------------------------- */
+
+/* Rows to 8-bit integers: dScale[t] = fl32(max_k |x[t,k]| / 127) and
+ * q[t,k] = x[t,k] / dScale[t], the real quotient rounded once to the nearest
+ * integer (ties to even) and clamped to [-127, 127]; a row of zeros (or one so
+ * small that its scale rounds to 0) has scale 0 and q = 0; a row with an
+ * infinity or NaN has scale NaN and q = 0. Applied to activations (T x K) the
+ * scales are per token, applied to a weight (N x K) per channel. Bytes of dQ
+ * beyond a row's K are not written.
+ * With dChecksum[K] (abft_column_checksum of the weight the rows will be
+ * multiplied with) the same pass encodes the product's expected row sums:
+ * dExpect[t] = sum_k q[t,k] * dChecksum[k], exact in 64 bits. Both or neither
+ * of dChecksum and dExpect. */
+int abft_quantize_rows(const void* dX, int64_t ldx, int type, int T, int K, int8_t* dQ, int64_t ldq, float* dScale,
+                       const int32_t* dChecksum, int64_t* dExpect, void* stream);
+
+/* dChecksum[k] = sum_n w[n,k] of an 8-bit weight, exact (N <= ABFT_INT8_MAX_ROWS).
+ * Taken once when a weight is loaded. */
+int abft_column_checksum(const int8_t* dW, int64_t ldw, int N, int K, int32_t* dChecksum, void* stream);
+
+/* y[t,n] = (sum_k q[t,k] * w[n,k]) * dQScale[t] * dWScale[n], the sum exact in
+ * 32 bits (K <= ABFT_INT8_MAX_K), the scales applied in 32-bit floating point
+ * in this order, rounded once to the type of dY.
+ * With dExpect[T] (from abft_quantize_rows) the product is verified while it
+ * is computed: dRowDiff[t] = sum_n sum_k q[t,k] * w[n,k] - dExpect[t], taken
+ * from the integer sums themselves. It is exactly 0 for every sound row: there
+ * is no threshold and there are no false alarms. A flipped bit in q or w since
+ * they were encoded, or in a sum, leaves a difference (faults whose effects on
+ * one row cancel are not seen; the scaling after the sums is not covered).
+ * Both or neither of dExpect and dRowDiff. */
+size_t abft_int8_matmul_ws_bytes(const int8_t* dQ, int64_t ldq, const int8_t* dW, int64_t ldw, int T, int N, int K);
+int abft_int8_matmul(const int8_t* dQ, int64_t ldq, const float* dQScale, const int8_t* dW, int64_t ldw,
+                     const float* dWScale, int T, int N, int K, void* dY, int64_t ldy, int type,
+                     const int64_t* dExpect, int64_t* dRowDiff, void* dWork, size_t work_bytes, void* stream);
+
+/* Gated feed-forward block: g = x Wgate^T, u = x Wup^T, h = act(g) * u, with x
+ * T x K, the weights N x K, all of one 16-bit type; sums and activation in 32
+ * bits, h rounded once. With dG and dU (both or neither) g and u are kept for
+ * the backward pass, each rounded once. */
+size_t abft_gated_ffn_ws_bytes(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg, const void* dWUp,
+                               int64_t ldwu, int T, int N, int K);
+int abft_gated_ffn(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg, const void* dWUp, int64_t ldwu,
+                   int T, int N, int K, int type, int activation, void* dH, int64_t ldh, void* dG, int64_t ldg,
+                   void* dU, int64_t ldu, void* dWork, size_t work_bytes, void* stream);
+
+/* Its gradients from dh (T x N) and the kept g, u:
+ *   dgate = dh * u * act'(g), dup = dh * act(g)   (rounded to the type: operands of the products)
+ *   dx = dgate Wgate + dup Wup (T x K), dWgate = dgate^T x, dWup = dup^T x (N x K)
+ * Sums in 32 bits, each gradient rounded once; they are written, not added. */
+size_t abft_gated_ffn_backward_ws_bytes(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg,
+                                        const void* dWUp, int64_t ldwu, int T, int N, int K);
+int abft_gated_ffn_backward(const void* dDH, int64_t ldd, const void* dX, int64_t ldx, const void* dWGate,
+                            int64_t ldwg, const void* dWUp, int64_t ldwu, const void* dG, int64_t ldg, const void* dU,
+                            int64_t ldu, int T, int N, int K, int type, int activation, void* dDX, int64_t lddx,
+                            void* dDWGate, int64_t lddwg, void* dDWUp, int64_t lddwu, void* dWork, size_t work_bytes,
+                            void* stream);
 
 /* ------------------------------------------------------------------------
  * Session: one rank's online pipeline (pipeline/passes.cuh, buffers.cuh).
