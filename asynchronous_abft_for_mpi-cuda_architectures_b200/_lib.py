@@ -129,6 +129,7 @@ SIGNATURES = {
     "abft_inject_add": (_I, [_P, _I64, _I, _I, _F, _P]),
     "abft_inject_bitflip": (_I, [_P, _I64, _I, _I, _I, _P]),
     "abft_sgemm": (_I, [_P, _P, _I, _P, _I, _P, _I, _I, _I, _I]),
+    "abft_products_status": (_I, [_IP]),
     "abft_quantize_rows": (_I, [_P, _I64, _I, _I, _I, _P, _I64, _P, _P, _P, _P]),
     "abft_column_checksum": (_I, [_P, _I64, _I, _I, _P, _P]),
     "abft_int8_matmul_ws_bytes": (_Z, [_P, _I64, _P, _I64, _I, _I, _I]),

@@ -43,6 +43,7 @@
 
 #include "abft_b200.h"
 #include "abft_internal.h"
+#include "abft_tensor.h"
 
 namespace abft {
 namespace {
@@ -1698,6 +1699,10 @@ int set_verify_kernel(int which) {
 }
 
 int verify_kernel() { return g_verify_kernel.load(std::memory_order_relaxed); }
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() { return tensor_map_encoder(); }
+
+int wait_limit() { return g_wait_limit.load(); }
 
 int set_wait_limit(int polls) {
     if (polls < 0) return -1;

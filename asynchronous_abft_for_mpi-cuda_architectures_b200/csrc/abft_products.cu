@@ -9,14 +9,19 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "abft_b200.h"
 #include "abft_internal.h"
+#include "abft_tensor.h"
 
 namespace abft {
 namespace {
+
+constexpr int kWaitLimit = 1 << 20;  // polls of the waits that follow one that ran out
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
@@ -137,57 +142,332 @@ __global__ void __launch_bounds__(256) k_column_checksum(const int8_t* __restric
 }
 
 // ---------------------------------------------------------------- products ---
+//
+// One persistent kernel for all products, D = A B^T in tiles of 128 CG rows x
+// BN columns of sums, on the tcgen05 tensor cores:
+//
+//   kInt8   q w^T, scaled                      A: q [T, K]       B: w [N, K]
+//   kGate   act(x Wg^T) * (x Wu^T)             A: x [T, K]       B: Wg | Wu, BN / 2 rows each
+//   kDx     dg Wg + du Wu                      A: dg, du [T, N]  B: Wg, Wu read along their rows (MN-major)
+//   kDw     dg^T x and du^T x                  A: dg or du       B: x, both MN-major
+//
+// Warp 0 copies operand tiles to shared memory (TMA, 128-byte swizzle), one
+// thread of warp 1 issues the matrix instructions, warps 4-7 take finished
+// sums out of tensor memory; sums are double-buffered there, so the next
+// tile's products run while this one is written. With CG = 2 two CTAs (two
+// SMs) form one 256-row tile: each holds its 128 rows of A and half of B, and
+// the matrix instruction of the leader reads both halves, which halves the
+// copies of B per product.
+//
+// Nothing is transposed in memory: an operand whose summed index runs along
+// the pitch is MN-major, which the matrix instructions read directly. Rows and
+// columns beyond a matrix are filled with zeros by the copies, so ragged sizes
+// take the same path; sums along K of zeros change nothing.
 
-constexpr int kTile = 64, kStep = 16;
+enum { kInt8, kGate, kDx, kDw };
 
-// One 64 x 64 tile of A B^T per block, operands by element strides: A(m, k) at
-// m * ar + k * ac, B(n, k) at n * br + k * bc.
-template <typename T, typename Acc>
-__device__ __forceinline__ void tile_product(const T* A, int64_t ar, int64_t ac, const T* B, int64_t br, int64_t bc,
-                                             int M, int N, int K, int m0, int n0, Acc (&acc)[4][4]) {
-    __shared__ Acc sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-    const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;
-    for (int k0 = 0; k0 < K; k0 += kStep) {
-        for (int e = threadIdx.x; e < kTile * kStep; e += 256) {
-            const int r = e / kStep, k = e % kStep;
-            Acc a = 0, b = 0;
-            if constexpr (sizeof(T) == 1) {
-                if (m0 + r < M && k0 + k < K) a = A[(m0 + r) * ar + (k0 + k) * ac];
-                if (n0 + r < N && k0 + k < K) b = B[(n0 + r) * br + (k0 + k) * bc];
-            } else {
-                if (m0 + r < M && k0 + k < K) a = to_f32(A[(m0 + r) * ar + (k0 + k) * ac]);
-                if (n0 + r < N && k0 + k < K) b = to_f32(B[(n0 + r) * br + (k0 + k) * bc]);
-            }
-            sa[k][r] = a;
-            sb[k][r] = b;
+struct ProductArgs {
+    int rows, cols;              // of one output
+    int tiles_m, tiles_n;        // kDw: tiles_m counts both outputs' tiles
+    int tiles_m1;                // of the first output
+    int chunks;                  // of 128 bytes along K, one operand pair
+    int limit;                   // polls of a wait
+    void* c[3];                  // outputs; kGate: h, g, u; kDw: dWg, dWu
+    int64_t ld[3];
+    bool wide[3];                // 16-byte stores are possible
+    const float* row_scale;
+    const float* col_scale;
+    unsigned long long* rowdiff;
+};
+
+struct ProductMaps {
+    CUtensorMap a[2], b[2];
+};
+
+// Waits that ran out since the last abft_products_status, any product kernel of the device.
+__device__ unsigned g_fault;
+
+template <int MODE, int CG, int BN>
+struct Shape {
+    static constexpr bool kTwoPairs = MODE == kDx;
+    static constexpr bool kAMn = MODE == kDw;
+    static constexpr bool kBMn = MODE == kDx || MODE == kDw;
+    static constexpr int kARows = 128;                 // per CTA
+    static constexpr int kBRows = BN / CG;             // per CTA
+    static constexpr int kStageBytes = (kARows + kBRows) * 128;
+    static constexpr int kStages = (BN == 256 && CG == 1) ? 4 : (BN <= 64 ? 8 : 6);
+    static constexpr int kStagesEnd = kStages * kStageBytes;
+    static constexpr int kBars = kStagesEnd + 4 * 256 * 4;  // after the epilogue warps' scales
+    static constexpr int kSmem = 1024 + kBars + 512;
+    static constexpr int kOutCols = MODE == kGate ? BN / 2 : BN;
+    static constexpr int kTmemCols = 2 * BN;
+    static constexpr int kChunk = MODE == kInt8 ? 128 : 64;  // elements of 128 bytes
+};
+
+// A wait with a limit. `stop` is set for the whole CTA by the first that runs out.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, int limit, volatile int* stop) {
+    for (int i = 0; i < limit; ++i) {
+        if (tensor::bar_test(bar, parity)) return true;
+        if ((i & 63) == 63 && *stop) return false;
+    }
+    if (!*stop) {
+        *stop = 1;
+        atomicExch(&g_fault, 1u);
+    }
+    return false;
+}
+
+// Tile order: groups of 8 tile rows, columns inside a group, so that the CTAs
+// at work at one time read few operand rows (L2 hits).
+__device__ __forceinline__ void tile_at(int i, int tiles_m, int tiles_n, int& m, int& n) {
+    const int group = 8 * tiles_n;
+    const int g = i / group, r = i - g * group;
+    const int h = min(8, tiles_m - g * 8);
+    n = r / h;
+    m = g * 8 + r - n * h;
+}
+
+// 32 values to row `row` of a matrix from column n on.
+template <typename O>
+__device__ __forceinline__ void store32(O* row, int n, int cols, bool wide, const float (&v)[32]) {
+    constexpr int kV = 16 / sizeof(O);
+#pragma unroll
+    for (int j = 0; j < 32; j += kV) {
+        if (wide && n + j + kV <= cols) {
+            alignas(16) O pack[kV];
+#pragma unroll
+            for (int i = 0; i < kV; ++i) pack[i] = from_f32<O>(v[j + i]);
+            *reinterpret_cast<uint4*>(row + n + j) = *reinterpret_cast<uint4*>(pack);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kV; ++i)
+                if (n + j + i < cols) row[n + j + i] = from_f32<O>(v[j + i]);
         }
-        __syncthreads();
-        for (int k = 0; k < kStep; ++k)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) acc[i][j] += sa[k][tm * 4 + i] * sb[k][tn * 4 + j];
-        __syncthreads();
     }
 }
 
-template <typename O>
-__global__ void __launch_bounds__(256) k_int8_matmul(const int8_t* q, int64_t ldq, const float* q_scale,
-                                                     const int8_t* w, int64_t ldw, const float* w_scale, int T, int N,
-                                                     int K, O* y, int64_t ldy, unsigned long long* rowdiff) {
-    int acc[4][4] = {};
-    const int m0 = blockIdx.y * kTile, n0 = blockIdx.x * kTile;
-    tile_product<int8_t, int>(q, ldq, 1, w, ldw, 1, T, N, K, m0, n0, acc);
-    for (int i = 0; i < 4; ++i) {
-        const int t = m0 + threadIdx.x / 16 * 4 + i;
-        if (t >= T) continue;
-        long long sum = 0;
-        for (int j = 0; j < 4; ++j) {
-            const int n = n0 + threadIdx.x % 16 * 4 + j;
-            if (n >= N) continue;
-            sum += acc[i][j];
-            y[t * ldy + n] = from_f32<O>(static_cast<float>(acc[i][j]) * q_scale[t] * w_scale[n]);
+template <int MODE, int CG, int BN, typename O, int ACT>
+__global__ void __launch_bounds__(256, 1) k_product(const __grid_constant__ ProductMaps maps, const ProductArgs a) {
+    using S = Shape<MODE, CG, BN>;
+    extern __shared__ char raw[];
+    char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    const uint32_t base = tensor::smem_u32(smem);
+    float* scales = reinterpret_cast<float*>(smem + S::kStagesEnd);
+    const uint32_t bars = base + S::kBars;
+    auto full = [&](int s) { return bars + 8 * s; };
+    auto empty = [&](int s) { return bars + 8 * (S::kStages + s); };
+    auto sums_full = [&](int s) { return bars + 8 * (2 * S::kStages + s); };
+    auto sums_empty = [&](int s) { return bars + 8 * (2 * S::kStages + 2 + s); };
+    const uint32_t drained = bars + 8 * (2 * S::kStages + 4);
+    volatile int* stop = reinterpret_cast<volatile int*>(smem + S::kBars + 8 * (2 * S::kStages + 5));
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(const_cast<int*>(stop) + 1);
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = CG == 2 ? tensor::cluster_rank() : 0;
+    const int tiles = a.tiles_m * a.tiles_n;
+    const int first = blockIdx.x / CG, step = gridDim.x / CG;
+    const int chunks = S::kTwoPairs ? 2 * a.chunks : a.chunks;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) {
+            tensor::bar_init(full(s), 1);
+            tensor::bar_init(empty(s), 1);
         }
-        if (rowdiff) atomicAdd(rowdiff + t, static_cast<unsigned long long>(sum));
+        for (int s = 0; s < 2; ++s) {
+            tensor::bar_init(sums_full(s), 1);
+            tensor::bar_init(sums_empty(s), 4 * CG);
+        }
+        tensor::bar_init(drained, 1);
+        *stop = 0;
+        tensor::bar_init_fence();
     }
+    if (warp == 2) tensor::tmem_alloc<CG>(tensor::smem_u32(const_cast<uint32_t*>(tmem_slot)), S::kTmemCols);
+    tensor::tc_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) tensor::cluster_sync();
+    tensor::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0 && lane == 0) {
+        // ------------------------------------------------ copies ---
+        for (int i = 0; i < 2; ++i) {
+            tensor::prefetch_map(&maps.a[i]);
+            tensor::prefetch_map(&maps.b[i]);
+        }
+        int it = 0;
+        bool ok = true;
+        for (int tile = first; ok && tile < tiles; tile += step) {
+            int mt, nt;
+            tile_at(tile, a.tiles_m, a.tiles_n, mt, nt);
+            int pair = 0;
+            if (MODE == kDw && mt >= a.tiles_m1) {
+                mt -= a.tiles_m1;
+                pair = 1;
+            }
+            const int m0 = (mt * CG + (int)rank) * 128;
+            const int n0 = MODE == kGate ? nt * S::kOutCols : nt * BN + (int)rank * S::kBRows;
+            for (int c = 0; c < chunks; ++c, ++it) {
+                const int s = it % S::kStages;
+                if (!wait_for(empty(s), (it / S::kStages + 1) & 1, a.limit, stop)) {
+                    ok = false;
+                    break;
+                }
+                if (rank == 0) tensor::bar_expect(full(s), CG * S::kStageBytes);
+                const uint32_t done = CG == 2 ? tensor::in_leader(full(s)) : full(s);
+                const uint32_t sa = base + s * S::kStageBytes, sb = sa + S::kARows * 128;
+                int k = c;
+                if constexpr (S::kTwoPairs) {
+                    pair = c >= a.chunks;
+                    k = pair ? c - a.chunks : c;
+                }
+                const CUtensorMap* am = &maps.a[pair];
+                if constexpr (S::kAMn) {
+                    tensor::tma_load<CG>(sa, am, m0, k * 64, done);
+                    tensor::tma_load<CG>(sa + 8192, am, m0 + 64, k * 64, done);
+                } else {
+                    tensor::tma_load<CG>(sa, am, k * S::kChunk, m0, done);
+                }
+                if constexpr (S::kBMn) {
+                    const CUtensorMap* bm = MODE == kDx ? &maps.b[pair] : &maps.b[0];
+#pragma unroll
+                    for (int j = 0; j < S::kBRows / 64; ++j)
+                        tensor::tma_load<CG>(sb + j * 8192, bm, n0 + j * 64, k * 64, done);
+                } else if constexpr (MODE == kGate && CG == 2) {
+                    tensor::tma_load<CG>(sb, &maps.b[rank], k * S::kChunk, n0, done);
+                } else if constexpr (MODE == kGate) {
+                    tensor::tma_load<CG>(sb, &maps.b[0], k * S::kChunk, n0, done);
+                    tensor::tma_load<CG>(sb + BN / 2 * 128, &maps.b[1], k * S::kChunk, n0, done);
+                } else {
+                    tensor::tma_load<CG>(sb, &maps.b[0], k * S::kChunk, n0, done);
+                }
+            }
+        }
+        // The CTA stays until the last stages are read (the pair's leader signals both CTAs).
+        for (int j = max(0, it - S::kStages); ok && j < it; ++j)
+            ok = wait_for(empty(j % S::kStages), (j / S::kStages) & 1, a.limit, stop);
+        if (!ok) {  // after a wait that ran out the copies in flight land first
+            if (rank == 0)
+                for (int j = max(0, it - S::kStages); j < it; ++j)
+                    for (int i = 0; i < kWaitLimit && !tensor::bar_test(full(j % S::kStages), (j / S::kStages) & 1); ++i) {
+                    }
+            else
+                for (int i = 0; i < 1000 && it > 0; ++i) __nanosleep(1000);
+        }
+    } else if (warp == 1 && lane == 0) {
+        // ------------------------------------- matrix instructions ---
+        constexpr uint32_t idesc =
+            tensor::instruction(128 * CG, BN, MODE == kInt8, std::is_same<O, __nv_bfloat16>::value, S::kAMn, S::kBMn);
+        constexpr uint32_t a_step = S::kAMn ? 2048 >> 4 : 32 >> 4, b_step = S::kBMn ? 2048 >> 4 : 32 >> 4;
+        int it = 0, n = 0;
+        bool ok = true;
+        for (int tile = first; rank == 0 && ok && tile < tiles; tile += step, ++n) {
+            const int buf = n & 1;
+            if (!wait_for(sums_empty(buf), ((n >> 1) + 1) & 1, a.limit, stop)) break;
+            tensor::tc_fence_after();
+            const uint32_t d = tmem + buf * BN;
+            for (int c = 0; c < chunks; ++c, ++it) {
+                const int s = it % S::kStages;
+                if (!wait_for(full(s), (it / S::kStages) & 1, a.limit, stop)) {
+                    ok = false;
+                    break;
+                }
+                tensor::tc_fence_after();
+                const uint32_t sa = base + s * S::kStageBytes;
+                const uint64_t da = tensor::operand(sa, S::kAMn), db = tensor::operand(sa + S::kARows * 128, S::kBMn);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    tensor::mma<CG, MODE == kInt8>(d, da + k * a_step, db + k * b_step, idesc, c > 0 || k > 0);
+                tensor::mma_commit<CG>(empty(s));
+            }
+            if (ok) tensor::mma_commit<CG>(sums_full(buf));
+        }
+        // instructions in flight still read shared and write tensor memory, in both CTAs of a pair
+        if (rank == 0) tensor::mma_commit<CG>(drained);
+        for (int i = 0; i < kWaitLimit && !tensor::bar_test(drained, 0); ++i) {
+        }
+    } else if (warp >= 4) {
+        // -------------------------------------------------- results ---
+        const int w = warp - 4;
+        const uint32_t lanes = tmem + ((uint32_t)w << 21);
+        int n = 0;
+        for (int tile = first; tile < tiles; tile += step, ++n) {
+            const int buf = n & 1;
+            int mt, nt;
+            tile_at(tile, a.tiles_m, a.tiles_n, mt, nt);
+            int out = 0;
+            if (MODE == kDw && mt >= a.tiles_m1) {
+                mt -= a.tiles_m1;
+                out = 1;
+            }
+            const int m = (mt * CG + (int)rank) * 128 + w * 32 + lane;
+            const int n0 = nt * S::kOutCols;
+            const bool live = m < a.rows;
+            float* sc = scales + w * 256;
+            float rs = 0.0f;
+            if constexpr (MODE == kInt8) {
+                __syncwarp();
+                for (int j = lane; j < BN; j += 32) sc[j] = n0 + j < a.cols ? a.col_scale[n0 + j] : 0.0f;
+                if (live) rs = a.row_scale[m];
+                __syncwarp();
+            }
+            if (!__all_sync(~0u, wait_for(sums_full(buf), (n >> 1) & 1, a.limit, stop))) break;
+            tensor::tc_fence_after();
+            long long total = 0;
+#pragma unroll 1
+            for (int j = 0; j < S::kOutCols; j += 32) {
+                uint32_t r[32], r2[32];
+                __syncwarp();
+                tensor::tmem_load32(lanes + buf * BN + j, r);
+                if constexpr (MODE == kGate) tensor::tmem_load32(lanes + buf * BN + BN / 2 + j, r2);
+                tensor::tmem_wait_load(r);
+                if constexpr (MODE == kGate) tensor::after_wait(r2);
+                if (j + 32 == S::kOutCols) {  // the sums are out: the next tile may overwrite them
+                    tensor::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0)
+                        tensor::bar_arrive_cluster(CG == 2 ? tensor::in_leader(sums_empty(buf)) : sums_empty(buf));
+                }
+                if (live) {
+                    float v[32];
+                    if constexpr (MODE == kInt8) {
+    #pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const int sum = static_cast<int>(r[i]);
+                            total += sum;
+                            v[i] = static_cast<float>(sum) * rs * sc[j + i];
+                        }
+                        store32<O>(reinterpret_cast<O*>(a.c[0]) + m * a.ld[0], n0 + j, a.cols, a.wide[0], v);
+                    } else if constexpr (MODE == kGate) {
+                        float u[32];
+    #pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            v[i] = __uint_as_float(r[i]);
+                            u[i] = __uint_as_float(r2[i]);
+                        }
+                        if (a.c[1]) {
+                            store32<O>(reinterpret_cast<O*>(a.c[1]) + m * a.ld[1], n0 + j, a.cols, a.wide[1], v);
+                            store32<O>(reinterpret_cast<O*>(a.c[2]) + m * a.ld[2], n0 + j, a.cols, a.wide[2], u);
+                        }
+    #pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = act<ACT>(v[i]) * u[i];
+                        store32<O>(reinterpret_cast<O*>(a.c[0]) + m * a.ld[0], n0 + j, a.cols, a.wide[0], v);
+                    } else {
+    #pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+                        store32<O>(reinterpret_cast<O*>(a.c[out]) + m * a.ld[out], n0 + j, a.cols, a.wide[out], v);
+                    }
+                }
+            }
+            if (MODE == kInt8 && live && a.rowdiff)
+                atomicAdd(a.rowdiff + m, static_cast<unsigned long long>(total));
+        }
+    }
+    __syncwarp();
+    tensor::tc_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) tensor::cluster_sync();
+    tensor::tc_fence_after();
+    if (warp == 2) tensor::tmem_free<CG>(tmem, S::kTmemCols);
 }
 
 __global__ void k_negate(const int64_t* __restrict__ in, int64_t* __restrict__ out, int n) {
@@ -195,24 +475,13 @@ __global__ void k_negate(const int64_t* __restrict__ in, int64_t* __restrict__ o
     if (i < n) out[i] = -in[i];
 }
 
-template <typename T, int ACT>
-__global__ void __launch_bounds__(256) k_gated_ffn(const T* x, int64_t ldx, const T* wg, int64_t ldwg, const T* wu,
-                                                   int64_t ldwu, int Tn, int N, int K, T* h, int64_t ldh, T* gs,
-                                                   int64_t ldg, T* us, int64_t ldu) {
-    float g[4][4] = {}, u[4][4] = {};
-    const int m0 = blockIdx.y * kTile, n0 = blockIdx.x * kTile;
-    tile_product<T, float>(x, ldx, 1, wg, ldwg, 1, Tn, N, K, m0, n0, g);
-    tile_product<T, float>(x, ldx, 1, wu, ldwu, 1, Tn, N, K, m0, n0, u);
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int64_t t = m0 + threadIdx.x / 16 * 4 + i, n = n0 + threadIdx.x % 16 * 4 + j;
-            if (t >= Tn || n >= N) continue;
-            h[t * ldh + n] = from_f32<T>(act<ACT>(g[i][j]) * u[i][j]);
-            if (gs) {
-                gs[t * ldg + n] = from_f32<T>(g[i][j]);
-                us[t * ldu + n] = from_f32<T>(u[i][j]);
-            }
-        }
+// Copies rows onto a pitch of 16 bytes.
+template <typename T>
+__global__ void __launch_bounds__(256) k_pack(const T* __restrict__ in, int64_t ld, int rows, int cols, T* __restrict__ out,
+                                              int64_t ldo) {
+    const int c = blockIdx.y * 256 + threadIdx.x;
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
+        if (c < cols) out[r * ldo + c] = in[r * ld + c];
 }
 
 template <typename T, int ACT>
@@ -228,23 +497,9 @@ __global__ void __launch_bounds__(256) k_gate_grad(const T* dh, int64_t ldd, con
     du[t * ldo + n] = from_f32<T>(d * a);
 }
 
-// C = A0 B0^T (+ A1 B1^T)
-template <typename T>
-__global__ void __launch_bounds__(256) k_product(const T* A0, const T* A1, int64_t ar, int64_t ac, const T* B0,
-                                                 int64_t br0, int64_t bc0, const T* B1, int64_t br1, int64_t bc1,
-                                                 int M, int N, int K, T* C, int64_t ldc) {
-    float acc[4][4] = {};
-    const int m0 = blockIdx.y * kTile, n0 = blockIdx.x * kTile;
-    tile_product<T, float>(A0, ar, ac, B0, br0, bc0, M, N, K, m0, n0, acc);
-    if (A1) tile_product<T, float>(A1, ar, ac, B1, br1, bc1, M, N, K, m0, n0, acc);
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int64_t m = m0 + threadIdx.x / 16 * 4 + i, n = n0 + threadIdx.x % 16 * 4 + j;
-            if (m < M && n < N) C[m * ldc + n] = from_f32<T>(acc[i][j]);
-        }
-}
+// -------------------------------------------------------------------- host ---
 
-int cdiv(int a, int b) { return (a + b - 1) / b; }
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 int bad(const char* msg) {
     set_error(msg);
@@ -256,8 +511,111 @@ int launched(const char* what) {
     return e == cudaSuccess ? ABFT_OK : cuda_fail(e, what);
 }
 
+// A row-major operand of elements of `size` bytes. One that bulk tensor copies
+// cannot read (base or pitch not a multiple of 16 bytes) is copied first.
+struct Operand {
+    const void* p;
+    int64_t ld;
+    int rows, cols, size;
+
+    bool direct() const { return ((uintptr_t)p & 15) == 0 && (rows == 1 || (ld * size & 15) == 0); }
+    int64_t packed_pitch() const { return cdiv((int64_t)cols * size, 16) * 16 / size; }
+    size_t bytes() const { return direct() ? 0 : ((size_t)rows * packed_pitch() * size + 255) & ~(size_t)255; }
+
+    // In place of an operand that is not direct, its copy in `work`, which moves on.
+    void pack(char*& work, cudaStream_t s) {
+        if (direct()) return;
+        const dim3 grid((unsigned)std::min<int64_t>(rows, 4096), (unsigned)cdiv(cols, 256));
+        if (size == 1)
+            k_pack<<<grid, 256, 0, s>>>((const int8_t*)p, ld, rows, cols, (int8_t*)work, packed_pitch());
+        else
+            k_pack<<<grid, 256, 0, s>>>((const uint16_t*)p, ld, rows, cols, (uint16_t*)work, packed_pitch());
+        const size_t n = bytes();
+        p = work;
+        ld = packed_pitch();
+        work += n;
+    }
+
+    // Boxes of 128 bytes x box_rows.
+    bool map(CUtensorMap* m, int box_rows) const {
+        auto enc = encode_tiled();
+        if (!enc) return false;
+        const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+        const cuuint64_t strides[1] = {(cuuint64_t)(rows == 1 ? packed_pitch() : ld) * size};
+        const cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows};
+        const cuuint32_t one[2] = {1, 1};
+        return enc(m, size == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(p),
+                   dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    }
+};
+
+// Number of SMs of the current device.
+int sm_count() {
+    static std::atomic<int> cache[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+    if (dev >= 0 && dev < 64 && cache[dev].load()) return cache[dev].load();
+    int n = 148;
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (dev >= 0 && dev < 64) cache[dev].store(n);
+    return n;
+}
+
+template <int MODE, int CG, int BN, typename O, int ACT>
+int launch_product(const Operand (&a)[2], const Operand (&b)[2], ProductArgs args, const char* name, cudaStream_t s) {
+    using S = Shape<MODE, CG, BN>;
+    ProductMaps maps;
+    const int b_box = S::kBMn ? 64 : MODE == kGate ? BN / 2 : S::kBRows;
+    const int a_box = S::kAMn ? 64 : 128;
+    bool made = a[0].map(&maps.a[0], a_box) && b[0].map(&maps.b[0], b_box);
+    maps.a[1] = maps.a[0];
+    maps.b[1] = maps.b[0];
+    if (made && a[1].p != a[0].p) made = a[1].map(&maps.a[1], a_box);
+    if (made && b[1].p != b[0].p) made = b[1].map(&maps.b[1], b_box);
+    if (!made) {
+        set_error(std::string(name) + ": a tensor map could not be made");
+        return ABFT_ERR_CUDA;
+    }
+    args.tiles_m1 = (int)cdiv(args.rows, 128 * CG);
+    args.tiles_m = MODE == kDw ? 2 * args.tiles_m1 : args.tiles_m1;
+    args.tiles_n = (int)cdiv(args.cols, S::kOutCols);
+    args.limit = wait_limit();
+    for (int i = 0; i < 3; ++i)
+        args.wide[i] = ((uintptr_t)args.c[i] & 15) == 0 && (args.ld[i] * (int64_t)sizeof(O) & 15) == 0;
+    auto kernel = k_product<MODE, CG, BN, O, ACT>;
+    cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    if (e != cudaSuccess) return cuda_fail(e, name);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(std::min<int64_t>((int64_t)args.tiles_m * args.tiles_n, sm_count() / CG) * CG));
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, maps, args);
+    return e == cudaSuccess ? ABFT_OK : cuda_fail(e, name);
+}
+
+// CTAs of one tile and columns of sums: pairs of SMs with the widest tile for
+// enough tiles to fill the GPU, single ones with narrower tiles below that.
+template <int MODE, typename O, int ACT = 0>
+int product(const Operand (&a)[2], const Operand (&b)[2], const ProductArgs& args, const char* name, cudaStream_t s) {
+    const int64_t outputs = MODE == kDw ? 2 : 1, width = MODE == kGate ? 2 : 1;
+    const int64_t rows = outputs * cdiv(args.rows, 128);
+    if (outputs * cdiv(args.rows, 256) * cdiv(args.cols * width, 256) >= 4)
+        return launch_product<MODE, 2, 256, O, ACT>(a, b, args, name, s);
+    if (rows * cdiv(args.cols * width, 128) >= 2) return launch_product<MODE, 1, 128, O, ACT>(a, b, args, name, s);
+    return launch_product<MODE, 1, 64, O, ACT>(a, b, args, name, s);
+}
+
 // dgate | dup, each T rows on a pitch of 16 bytes
 int64_t grad_pitch(int N) { return (static_cast<int64_t>(N) + 7) / 8 * 8; }
+size_t grad_bytes(int T, int N) { return (static_cast<size_t>(T) * grad_pitch(N) * 2 + 255) & ~(size_t)255; }
 
 template <typename F>
 int with_type(int type, F&& f) {
@@ -299,12 +657,13 @@ int abft_quantize_rows(const void* dX, int64_t ldx, int type, int T, int K, int8
 int abft_column_checksum(const int8_t* dW, int64_t ldw, int N, int K, int32_t* dChecksum, void* stream) {
     if (!dW || !dChecksum || N < 1 || N > ABFT_INT8_MAX_ROWS || K < 1 || ldw < K)
         return bad("abft_column_checksum: bad argument (need pointers, 1 <= N <= 2^24, K >= 1, ldw >= K)");
-    k_column_checksum<<<cdiv(K, 256), 256, 0, (cudaStream_t)stream>>>(dW, ldw, N, K, dChecksum);
+    k_column_checksum<<<(unsigned)cdiv(K, 256), 256, 0, (cudaStream_t)stream>>>(dW, ldw, N, K, dChecksum);
     return launched("abft_column_checksum");
 }
 
 size_t abft_int8_matmul_ws_bytes(const int8_t* dQ, int64_t ldq, const int8_t* dW, int64_t ldw, int T, int N, int K) {
-    return 0;
+    if (T < 1 || N < 1 || K < 1) return 0;
+    return Operand{dQ, ldq, T, K, 1}.bytes() + Operand{dW, ldw, N, K, 1}.bytes();
 }
 
 int abft_int8_matmul(const int8_t* dQ, int64_t ldq, const float* dQScale, const int8_t* dW, int64_t ldw,
@@ -319,12 +678,22 @@ int abft_int8_matmul(const int8_t* dQ, int64_t ldq, const float* dQScale, const 
         return bad("abft_int8_matmul: bad argument (missing pointer, or one of dExpect and dRowDiff alone)");
     if (work_bytes < abft_int8_matmul_ws_bytes(dQ, ldq, dW, ldw, T, N, K)) return bad("abft_int8_matmul: workspace too small");
     cudaStream_t s = (cudaStream_t)stream;
-    if (dExpect) k_negate<<<cdiv(T, 256), 256, 0, s>>>(dExpect, dRowDiff, T);
+    if (dExpect) k_negate<<<(unsigned)cdiv(T, 256), 256, 0, s>>>(dExpect, dRowDiff, T);
+    Operand q{dQ, ldq, T, K, 1}, w{dW, ldw, N, K, 1};
+    char* work = (char*)dWork;
+    q.pack(work, s);
+    w.pack(work, s);
+    ProductArgs args = {};
+    args.rows = T;
+    args.cols = N;
+    args.chunks = (int)cdiv(K, 128);
+    args.c[0] = dY;
+    args.ld[0] = ldy;
+    args.row_scale = dQScale;
+    args.col_scale = dWScale;
+    args.rowdiff = (unsigned long long*)dRowDiff;
     auto go = [&](auto tag) {
-        using E = decltype(tag);
-        k_int8_matmul<E><<<dim3(cdiv(N, kTile), cdiv(T, kTile)), 256, 0, s>>>(
-            dQ, ldq, dQScale, dW, ldw, dWScale, T, N, K, (E*)dY, ldy, (unsigned long long*)dRowDiff);
-        return launched("abft_int8_matmul");
+        return product<kInt8, decltype(tag)>({q, q}, {w, w}, args, "abft_int8_matmul", s);
     };
     if (type == ABFT_TYPE_F32) return go(0.0f);
     return with_type(type, go);
@@ -332,7 +701,9 @@ int abft_int8_matmul(const int8_t* dQ, int64_t ldq, const float* dQScale, const 
 
 size_t abft_gated_ffn_ws_bytes(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg, const void* dWUp,
                                int64_t ldwu, int T, int N, int K) {
-    return 0;
+    if (T < 1 || N < 1 || K < 1) return 0;
+    return Operand{dX, ldx, T, K, 2}.bytes() + Operand{dWGate, ldwg, N, K, 2}.bytes() +
+           Operand{dWUp, ldwu, N, K, 2}.bytes();
 }
 
 int abft_gated_ffn(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg, const void* dWUp, int64_t ldwu,
@@ -348,13 +719,23 @@ int abft_gated_ffn(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg
         return bad("abft_gated_ffn: bad argument (missing pointer, or one of dG and dU alone)");
     if (work_bytes < abft_gated_ffn_ws_bytes(dX, ldx, dWGate, ldwg, dWUp, ldwu, T, N, K))
         return bad("abft_gated_ffn: workspace too small");
+    cudaStream_t s = (cudaStream_t)stream;
+    Operand x{dX, ldx, T, K, 2}, wg{dWGate, ldwg, N, K, 2}, wu{dWUp, ldwu, N, K, 2};
+    char* work = (char*)dWork;
+    x.pack(work, s);
+    wg.pack(work, s);
+    wu.pack(work, s);
+    ProductArgs args = {};
+    args.rows = T;
+    args.cols = N;
+    args.chunks = (int)cdiv(K, 64);
+    void* outs[3] = {dH, dG, dU};
+    const int64_t pitches[3] = {ldh, ldg, ldu};
+    std::copy(outs, outs + 3, args.c);
+    std::copy(pitches, pitches + 3, args.ld);
     return with_type(type, [&](auto tag) {
-        using E = decltype(tag);
         return with_act(activation, [&](auto a) {
-            k_gated_ffn<E, decltype(a)::value><<<dim3(cdiv(N, kTile), cdiv(T, kTile)), 256, 0, (cudaStream_t)stream>>>(
-                (const E*)dX, ldx, (const E*)dWGate, ldwg, (const E*)dWUp, ldwu, T, N, K, (E*)dH, ldh, (E*)dG, ldg,
-                (E*)dU, ldu);
-            return launched("abft_gated_ffn");
+            return product<kGate, decltype(tag), decltype(a)::value>({x, x}, {wg, wu}, args, "abft_gated_ffn", s);
         });
     });
 }
@@ -362,7 +743,7 @@ int abft_gated_ffn(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg
 size_t abft_gated_ffn_backward_ws_bytes(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg,
                                         const void* dWUp, int64_t ldwu, int T, int N, int K) {
     if (T < 1 || N < 1 || K < 1) return 0;
-    return 4 * static_cast<size_t>(T) * grad_pitch(N);
+    return 2 * grad_bytes(T, N) + abft_gated_ffn_ws_bytes(dX, ldx, dWGate, ldwg, dWUp, ldwu, T, N, K);
 }
 
 int abft_gated_ffn_backward(const void* dDH, int64_t ldd, const void* dX, int64_t ldx, const void* dWGate,
@@ -386,24 +767,48 @@ int abft_gated_ffn_backward(const void* dDH, int64_t ldd, const void* dX, int64_
         return bad("abft_gated_ffn_backward: bad argument (missing pointer)");
     if (!dWork || work_bytes < abft_gated_ffn_backward_ws_bytes(dX, ldx, dWGate, ldwg, dWUp, ldwu, T, N, K))
         return bad("abft_gated_ffn_backward: workspace too small");
+    const int64_t p = grad_pitch(N);
+    char* work = (char*)dWork;
+    const Operand dg{work, p, T, N, 2}, du{work + grad_bytes(T, N), p, T, N, 2};
+    work += 2 * grad_bytes(T, N);
+    Operand x{dX, ldx, T, K, 2}, wg{dWGate, ldwg, N, K, 2}, wu{dWUp, ldwu, N, K, 2};
+    x.pack(work, s);
+    wg.pack(work, s);
+    wu.pack(work, s);
     return with_type(type, [&](auto tag) {
         using E = decltype(tag);
-        const int64_t p = grad_pitch(N);
-        E* dg = (E*)dWork;
-        E* du = dg + T * p;
         with_act(activation, [&](auto a) {
-            k_gate_grad<E, decltype(a)::value><<<dim3(T, cdiv(N, 256)), 256, 0, s>>>(
-                (const E*)dDH, ldd, (const E*)dG, ldg, (const E*)dU, ldu, N, dg, du, p);
+            k_gate_grad<E, decltype(a)::value><<<dim3(T, (unsigned)cdiv(N, 256)), 256, 0, s>>>(
+                (const E*)dDH, ldd, (const E*)dG, ldg, (const E*)dU, ldu, N, (E*)dg.p, (E*)du.p, p);
             return 0;
         });
-        k_product<E><<<dim3(cdiv(K, kTile), cdiv(T, kTile)), 256, 0, s>>>(
-            dg, du, p, 1, (const E*)dWGate, 1, ldwg, (const E*)dWUp, 1, ldwu, T, K, N, (E*)dDX, lddx);
-        k_product<E><<<dim3(cdiv(K, kTile), cdiv(N, kTile)), 256, 0, s>>>(
-            dg, nullptr, 1, p, (const E*)dX, 1, ldx, nullptr, 0, 0, N, K, T, (E*)dDWGate, lddwg);
-        k_product<E><<<dim3(cdiv(K, kTile), cdiv(N, kTile)), 256, 0, s>>>(
-            du, nullptr, 1, p, (const E*)dX, 1, ldx, nullptr, 0, 0, N, K, T, (E*)dDWUp, lddwu);
+        ProductArgs args = {};
+        args.rows = T;
+        args.cols = K;
+        args.chunks = (int)cdiv(N, 64);
+        args.c[0] = dDX;
+        args.ld[0] = lddx;
+        if (int rc = product<kDx, E>({dg, du}, {wg, wu}, args, "abft_gated_ffn_backward", s)) return rc;
+        args.rows = N;
+        args.chunks = (int)cdiv(T, 64);
+        args.c[0] = dDWGate;
+        args.ld[0] = lddwg;
+        args.c[1] = dDWUp;
+        args.ld[1] = lddwu;
+        if (int rc = product<kDw, E>({dg, du}, {x, x}, args, "abft_gated_ffn_backward", s)) return rc;
         return launched("abft_gated_ffn_backward");
     });
+}
+
+int abft_products_status(int* fault) {
+    if (!fault) return bad("abft_products_status: fault is NULL");
+    unsigned f = 0;
+    const unsigned none = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&f, g_fault, sizeof(f));
+    if (e == cudaSuccess && f) e = cudaMemcpyToSymbol(g_fault, &none, sizeof(none));
+    if (e != cudaSuccess) return cuda_fail(e, "abft_products_status");
+    *fault = (int)f;
+    return ABFT_OK;
 }
 
 }  // extern "C"

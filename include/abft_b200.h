@@ -209,7 +209,8 @@ int abft_verify_noalloc(const float* dC_frag, int64_t ldc, int M, int N, const d
 int abft_set_verify_kernel(int which);
 
 /* Polls each wait of the TMA verify body makes for one bulk tensor copy
- * before it gives up (default 1048576). No counterpart in the reference, whose
+ * before it gives up (default 1048576; the waits inside the language-model
+ * products have the same limit, see abft_products_status). No counterpart in the reference, whose
  * kernels never wait on a copy. A wait that gives up marks the launch void:
  * the kernel waits (with the default limit) for the copies it issued, adds
  * nothing, finishes its arrival protocol and returns, and the next
@@ -262,6 +263,13 @@ int abft_sgemm(void* cublas_handle, const float* dA, int lda, const float* dB, i
  * Operands whose base or pitch is not a multiple of 16 bytes are supported;
  * they are copied into the workspace first.
  * ---------------------------------------------------------------------- */
+
+/* Synchronous: whether a wait inside a product kernel of the current device has
+ * run out since the last call (*fault = 1, then cleared). The kernels wait for
+ * their own copies and matrix instructions only, each wait with a limit
+ * (abft_set_wait_limit); after one that runs out they finish what is in
+ * flight, return, and the results of calls since the last status are void. */
+int abft_products_status(int* fault);
 
 /* Rows to 8-bit integers: dScale[t] = fl32(max_k |x[t,k]| / 127) and
  * q[t,k] = x[t,k] / dScale[t], the real quotient rounded once to the nearest
