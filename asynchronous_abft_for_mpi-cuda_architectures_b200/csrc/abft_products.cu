@@ -23,9 +23,6 @@ namespace {
 
 constexpr int kWaitLimit = 1 << 20;  // polls of the waits that follow one that ran out
 
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 
 template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
@@ -78,67 +75,263 @@ __device__ __forceinline__ void act_grad(float g, float& a, float& slope) {
 // -------------------------------------------------------- row quantisation ---
 //
 // scale = fl32(max |x| / 127), q = the real quotient x / scale rounded once to
-// the nearest integer, ties to even. The first guess x * (1 / scale) is off by
-// less than one step, and x - q scale is exact in 32 bits (both are multiples
-// of the same power of two and the difference has at most 24 bits), so
-// comparing twice it with the scale settles every tie.
-__device__ __forceinline__ float round_quotient(float x, float scale, float inv) {
-    float q = rintf(x * inv);
-    const float r2 = 2.0f * fmaf(-q, scale, x);
-    const float over = fabsf(r2) - scale;
-    const bool odd = (static_cast<int>(q) & 1) != 0;
-    if (over > 0.0f || (over == 0.0f && odd)) q += copysignf(1.0f, r2);
-    return fminf(fmaxf(q, -127.0f), 127.0f);
+// the nearest integer, ties to even. The first guess, x * (1 / scale) rounded,
+// is off by at most one and only where the quotient lies within 2^-16 of a
+// half; r = x - q scale is exact in 32 bits (both terms are multiples of the
+// same power of two and the difference has at most 24 bits), so comparing |r|
+// with scale / 2 settles it.
+//
+// Bound by reading x once: a row stays in registers between the search for its
+// maximum and its rounding. 5 instructions for an element's integer: adding
+// 1.5 * 2^23 rounds it and leaves it in the low byte, the remainder is only
+// checked for the largest of 8.
+constexpr float kRound = 12582912.0f;  // 1.5 * 2^23
+
+// The guess t = kRound + q moved by one where the quotient's half was missed.
+__device__ __forceinline__ float settle(float t, float x, float scale, float half) {
+    const float r = fmaf(-(t - kRound), scale, x);
+    const bool odd = (__float_as_int(t) & 1) != 0;
+    if (fabsf(r) > half || (fabsf(r) == half && odd)) t += copysignf(1.0f, r);
+    return t;
 }
 
+// Rows whose scale is near or below the smallest normal number: 2^100 times
+// everything is exact and keeps 1 / scale and the remainder normal; the scale
+// itself may have lost bits, so the quotient may pass 127.
+__device__ __noinline__ int quantize_tiny(float x, float scale) {
+    if (!(scale > 0.0f)) return 0;
+    const float s = scale * 0x1p100f;
+    x *= 0x1p100f;
+    const float q = fminf(fmaxf(rintf(x / s), -200.0f), 200.0f);
+    const float t = settle(q + kRound, fminf(fmaxf(x, -200.0f * s), 200.0f * s), s, 0.5f * s);
+    return static_cast<int>(fminf(fmaxf(t - kRound, -127.0f), 127.0f));
+}
+
+struct QuantArgs {
+    const void* x;
+    int64_t ldx;
+    int T, K;
+    int8_t* q;
+    int64_t ldq;
+    float* scale;
+    const int32_t* checksum;
+    int64_t* expect;
+};
+
+// Eight elements as they come from memory.
 template <typename T>
-__global__ void __launch_bounds__(256) k_quantize_rows(const T* __restrict__ x, int64_t ldx, int K, int8_t* __restrict__ q,
-                                                       int64_t ldq, float* __restrict__ scale,
-                                                       const int32_t* __restrict__ checksum,
-                                                       int64_t* __restrict__ expect) {
-    __shared__ unsigned smax[8];
-    __shared__ long long ssum[8];
-    const int row = blockIdx.x;
-    const T* xr = x + static_cast<int64_t>(row) * ldx;
-    int8_t* qr = q + static_cast<int64_t>(row) * ldq;
-    // largest magnitude by its bits: a NaN's are above infinity's, which are above every number's
-    unsigned m = 0;
-    for (int k = threadIdx.x; k < K; k += 256) m = max(m, __float_as_uint(to_f32(xr[k])) & 0x7fffffffu);
-    m = __reduce_max_sync(~0u, m);
-    if (threadIdx.x % 32 == 0) smax[threadIdx.x / 32] = m;
-    __syncthreads();
-    for (int w = 0; w < 8; ++w) m = max(m, smax[w]);
-    const bool finite = m < 0x7f800000u;
-    const float s = finite ? __fdiv_rn(__uint_as_float(m), 127.0f) : __uint_as_float(0x7fc00000u);
-    // 2^100 keeps 1 / scale and the remainder clear of the subnormal range
-    const float up = finite && s < 0x1p-100f ? 0x1p100f : 1.0f;
-    const float su = s * up;
-    const float inv = 1.0f / su;
-    long long sum = 0;
-    for (int k = threadIdx.x; k < K; k += 256) {
-        const int v = finite && s > 0.0f ? static_cast<int>(round_quotient(to_f32(xr[k]) * up, su, inv)) : 0;
-        qr[k] = static_cast<int8_t>(v);
-        if (checksum) sum += static_cast<long long>(v) * checksum[k];
+struct Eight {
+    uint4 v[sizeof(T) / 2];
+
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
     }
-    if (threadIdx.x == 0) scale[row] = s;
-    if (checksum) {
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-        if (threadIdx.x % 32 == 0) ssum[threadIdx.x / 32] = sum;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < 8; ++w) sum += ssum[w];
-            expect[row] = sum;
+    __device__ __forceinline__ void load(const T* p, int n) {  // n of them, zeros after
+        alignas(16) T e[8] = {};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) e[i] = p[i];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<uint4*>(e)[i];
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ float operator[](int i) const {
+        const uint32_t w = word(i * (int)sizeof(T) / 4);
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+            return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+        else return __half2float(__ushort_as_half((unsigned short)(i & 1 ? w >> 16 : w & 0xffffu)));
+    }
+    __device__ __forceinline__ uint32_t word(int i) const {
+        const uint4& q = v[i / 4];
+        return i % 4 == 0 ? q.x : i % 4 == 1 ? q.y : i % 4 == 2 ? q.z : q.w;
+    }
+    // Largest magnitude by its bits (a NaN's are above infinity's, which are above every number's), as a packed pair for
+    // the 16-bit types.
+    __device__ __forceinline__ uint32_t largest(uint32_t m) const {
+#pragma unroll
+        for (int i = 0; i < 2 * (int)sizeof(T); ++i) {
+            if constexpr (sizeof(T) == 4) m = max(m, word(i) & 0x7fffffffu);
+            else m = __vmaxu2(m, word(i) & 0x7fff7fffu);
+        }
+        return m;
+    }
+    // That largest as the bits of a 32-bit float.
+    static __device__ __forceinline__ uint32_t magnitude(uint32_t m) {
+        if constexpr (sizeof(T) == 4) return m;
+        const uint32_t h = max(m & 0xffffu, m >> 16);
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return h << 16;
+        else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+    }
+};
+
+// 8 integers of a row in two words.
+template <typename T>
+__device__ __forceinline__ uint2 quantize_eight(const Eight<T>& e, float scale, float inv, float half, bool normal) {
+    float t[8];
+    if (normal) {
+        float worst = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            t[i] = fmaf(e[i], inv, kRound);
+            worst = fmaxf(worst, fabsf(fmaf(-(t[i] - kRound), scale, e[i])));
+        }
+        if (worst >= half) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] = settle(t[i], e[i], scale, half);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = kRound + static_cast<float>(quantize_tiny(e[i], scale));
+    }
+    auto four = [&](int i) {
+        const uint32_t lo = __byte_perm(__float_as_uint(t[i]), __float_as_uint(t[i + 1]), 0x0040);
+        const uint32_t hi = __byte_perm(__float_as_uint(t[i + 2]), __float_as_uint(t[i + 3]), 0x0040);
+        return __byte_perm(lo, hi, 0x5410);
+    };
+    return make_uint2(four(0), four(4));
+}
+
+// One row per group of ROW threads, U pieces of 8 elements per thread, held in
+// registers; U = 0: any number of pieces, read twice. VEC: rows of x and the
+// checksum are 16-byte and rows of q 8-byte aligned. Groups walk the rows, so that the checksum's
+// pieces are loaded once.
+template <typename T, int ROW, int U, bool VEC>
+__global__ void __launch_bounds__(128) k_quantize_rows(const QuantArgs a) {
+    constexpr int kHeld = U > 0 ? U : 1;
+    constexpr bool kKeepSums = U > 0 && U <= 4;  // 8 registers of checksum a piece
+    __shared__ uint32_t smax[2][4];
+    __shared__ long long ssum[2][4];
+    const int me = threadIdx.x % ROW, groups = 128 / ROW;
+    const int pieces = (a.K + 7) / 8;
+    auto load = [&](Eight<T>& e, const T* row, int p) {
+        const int left = a.K - p * 8;
+        if (VEC && left >= 8) e.load(row + p * 8);
+        else if (left > 0) e.load(row + p * 8, left);
+        else e.zero();
+    };
+    auto checks = [&](int (&c)[8], int p) {
+        if (VEC && p * 8 + 8 <= a.K) {
+            const int4 lo = __ldg(reinterpret_cast<const int4*>(a.checksum + p * 8));
+            const int4 hi = __ldg(reinterpret_cast<const int4*>(a.checksum + p * 8) + 1);
+            c[0] = lo.x, c[1] = lo.y, c[2] = lo.z, c[3] = lo.w;
+            c[4] = hi.x, c[5] = hi.y, c[6] = hi.z, c[7] = hi.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i] = p * 8 + i < a.K ? a.checksum[p * 8 + i] : 0;
+        }
+    };
+    int c[kKeepSums ? U : 1][8];
+    if (kKeepSums && a.checksum) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) checks(c[u], me + u * ROW);
+    }
+    int flip = 0;
+    for (int64_t row = (int64_t)blockIdx.x * groups + threadIdx.x / ROW; row < a.T;
+         row += (int64_t)gridDim.x * groups, flip ^= 1) {
+        const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx;
+        int8_t* q = a.q + row * a.ldq;
+        Eight<T> e[kHeld];
+        uint32_t m = 0;
+        if constexpr (U > 0) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) load(e[u], x, me + u * ROW);
+#pragma unroll
+            for (int u = 0; u < U; ++u) m = e[u].largest(m);
+        } else {
+#pragma unroll 4
+            for (int p = me; p < pieces; p += ROW) {
+                Eight<T> v;
+                load(v, x, p);
+                m = v.largest(m);
+            }
+        }
+        m = __reduce_max_sync(~0u, Eight<T>::magnitude(m));
+        if constexpr (ROW == 128) {
+            if (threadIdx.x % 32 == 0) smax[flip][threadIdx.x / 32] = m;
+            __syncthreads();
+            m = max(max(smax[flip][0], smax[flip][1]), max(smax[flip][2], smax[flip][3]));
+        }
+        const bool finite = m < 0x7f800000u;
+        const float s = finite ? __fdiv_rn(__uint_as_float(m), 127.0f) : __uint_as_float(0x7fc00000u);
+        const bool normal = s >= 0x1p-100f;
+        const float inv = 1.0f / s, half = 0.5f * s;
+        long long sum = 0;
+        auto write = [&](const Eight<T>& v, int p, const int (&k)[8]) {
+            const int left = a.K - p * 8;
+            if (left <= 0) return;
+            const uint2 w = quantize_eight(v, s, inv, half, normal);
+            if (VEC && left >= 8) {
+                *reinterpret_cast<uint2*>(q + p * 8) = w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < left) q[p * 8 + i] = static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+            }
+            if (a.checksum) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    sum += (long long)static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3))) * k[i];
+            }
+        };
+        if constexpr (U > 0) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if constexpr (!kKeepSums)
+                    if (a.checksum) checks(c[0], me + u * ROW);
+                write(e[u], me + u * ROW, c[kKeepSums ? u : 0]);
+            }
+        } else {
+            for (int p = me; p < pieces; p += ROW) {
+                load(e[0], x, p);
+                if (a.checksum) checks(c[0], p);
+                write(e[0], p, c[0]);
+            }
+        }
+        if (me == 0) a.scale[row] = s;
+        if (a.checksum) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+            if constexpr (ROW == 128) {
+                if (threadIdx.x % 32 == 0) ssum[flip][threadIdx.x / 32] = sum;
+                __syncthreads();
+                sum = ssum[flip][0] + ssum[flip][1] + ssum[flip][2] + ssum[flip][3];
+            }
+            if (me == 0) a.expect[row] = sum;
         }
     }
 }
 
+// Column sums of an 8-bit weight: blocks of 256 rows, their sums added as
+// integers (the order does not matter). WIDE: 4 columns per load.
+template <bool WIDE>
 __global__ void __launch_bounds__(256) k_column_checksum(const int8_t* __restrict__ w, int64_t ldw, int N, int K,
                                                          int32_t* __restrict__ checksum) {
-    const int k = blockIdx.x * 256 + threadIdx.x;
+    constexpr int kC = WIDE ? 4 : 1;
+    const int64_t k = ((int64_t)blockIdx.x * 256 + threadIdx.x) * kC;
     if (k >= K) return;
-    int sum = 0;
-    for (int n = 0; n < N; ++n) sum += w[static_cast<int64_t>(n) * ldw + k];
-    checksum[k] = sum;
+    const int last = min(N, ((int)blockIdx.y + 1) * 256);
+    int sum[kC] = {};
+    if (WIDE && k + kC <= K) {
+#pragma unroll 8
+        for (int n = blockIdx.y * 256; n < last; ++n) {
+            const int v = __ldg(reinterpret_cast<const int*>(w + n * ldw + k));
+#pragma unroll
+            for (int i = 0; i < kC; ++i) sum[i] += static_cast<int8_t>(v >> (8 * i));
+        }
+    } else {
+        for (int n = blockIdx.y * 256; n < last; ++n)
+#pragma unroll
+            for (int i = 0; i < kC; ++i)
+                if (k + i < K) sum[i] += w[n * ldw + k + i];
+    }
+#pragma unroll
+    for (int i = 0; i < kC; ++i)
+        if (k + i < K) atomicAdd(checksum + k + i, sum[i]);
 }
 
 // ---------------------------------------------------------------- products ---
@@ -201,8 +394,7 @@ struct Shape {
     static constexpr int kSmem = 1024 + kBars + 512;
     static constexpr int kOutCols = MODE == kGate ? BN / 2 : BN;
     static constexpr int kTmemCols = 2 * BN;
-    static constexpr int kChunk = MODE == kInt8 ? 128 : 64;  // elements of 128 bytes
-};
+    };
 
 // A wait with a limit. `stop` is set for the whole CTA by the first that runs out.
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, int limit, volatile int* stop) {
@@ -267,6 +459,7 @@ __global__ void __launch_bounds__(256, 1) k_product(const __grid_constant__ Prod
     const int tiles = a.tiles_m * a.tiles_n;
     const int first = blockIdx.x / CG, step = gridDim.x / CG;
     const int chunks = S::kTwoPairs ? 2 * a.chunks : a.chunks;
+    constexpr int kElems = MODE == kInt8 ? 128 : 64;  // of 128 bytes along K
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) {
@@ -325,7 +518,7 @@ __global__ void __launch_bounds__(256, 1) k_product(const __grid_constant__ Prod
                     tensor::tma_load<CG>(sa, am, m0, k * 64, done);
                     tensor::tma_load<CG>(sa + 8192, am, m0 + 64, k * 64, done);
                 } else {
-                    tensor::tma_load<CG>(sa, am, k * S::kChunk, m0, done);
+                    tensor::tma_load<CG>(sa, am, k * kElems, m0, done);
                 }
                 if constexpr (S::kBMn) {
                     const CUtensorMap* bm = MODE == kDx ? &maps.b[pair] : &maps.b[0];
@@ -333,12 +526,12 @@ __global__ void __launch_bounds__(256, 1) k_product(const __grid_constant__ Prod
                     for (int j = 0; j < S::kBRows / 64; ++j)
                         tensor::tma_load<CG>(sb + j * 8192, bm, n0 + j * 64, k * 64, done);
                 } else if constexpr (MODE == kGate && CG == 2) {
-                    tensor::tma_load<CG>(sb, &maps.b[rank], k * S::kChunk, n0, done);
+                    tensor::tma_load<CG>(sb, &maps.b[rank], k * kElems, n0, done);
                 } else if constexpr (MODE == kGate) {
-                    tensor::tma_load<CG>(sb, &maps.b[0], k * S::kChunk, n0, done);
-                    tensor::tma_load<CG>(sb + BN / 2 * 128, &maps.b[1], k * S::kChunk, n0, done);
+                    tensor::tma_load<CG>(sb, &maps.b[0], k * kElems, n0, done);
+                    tensor::tma_load<CG>(sb + BN / 2 * 128, &maps.b[1], k * kElems, n0, done);
                 } else {
-                    tensor::tma_load<CG>(sb, &maps.b[0], k * S::kChunk, n0, done);
+                    tensor::tma_load<CG>(sb, &maps.b[0], k * kElems, n0, done);
                 }
             }
         }
@@ -470,6 +663,166 @@ __global__ void __launch_bounds__(256, 1) k_product(const __grid_constant__ Prod
     if (warp == 2) tensor::tmem_free<CG>(tmem, S::kTmemCols);
 }
 
+// ------------------------------------------------------------ few tokens ---
+//
+// Products of at most 32 tokens are bound by reading the weight once. The
+// 128-row tiles of the kernel above would leave most SMs without a tile and the
+// rest waiting on few copies, so here each block takes 16 weight rows (kGate: 8
+// of either weight) over all of K and its 8 warps share K: a warp reads 64 bytes
+// of 16 rows with 16-byte loads straight into the registers of the 16 x 8
+// matrix instruction (weights are its 16 rows, tokens its 8 columns). The sum
+// over K does not depend on the order of K, so lane t of a quad simply takes
+// the quad's t-th 16 bytes of a row, and of a token, as its part of K. Tokens
+// are re-read from L1. The warps' sums meet in shared memory, in a fixed order.
+
+template <bool INT8, typename E>
+__device__ __forceinline__ void few_mma(uint32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+#define ABFT_FEW(shape, types)                                                                                  \
+    asm volatile("mma.sync.aligned." shape ".row.col." types " {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, " \
+                 "{%0, %1, %2, %3};"                                                                            \
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])                                               \
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1))
+    if constexpr (INT8) ABFT_FEW("m16n8k32", "s32.s8.s8.s32");
+    else if constexpr (std::is_same<E, __half>::value) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    } else {
+        ABFT_FEW("m16n8k16", "f32.bf16.bf16.f32");
+    }
+#undef ABFT_FEW
+}
+
+struct FewArgs {
+    const char* w[2];  // kGate: both weights; else the weight in w[0]
+    int64_t ldw[2];    // bytes
+    const char* x;
+    int64_t ldx;       // bytes
+    int T, N;
+    int64_t kbytes;
+    void* c[3];
+    int64_t ld[3];
+    const float* row_scale;
+    const float* col_scale;
+    unsigned long long* rowdiff;
+};
+
+// 16 bytes at byte `off` of a row of `n` bytes, zeros beyond it; weights pass L1 by.
+template <bool STREAM>
+__device__ __forceinline__ uint4 few_load(const char* row, int64_t off) {
+    uint4 v;
+    if constexpr (STREAM)
+        asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "l"(row + off));
+    else
+        v = __ldg(reinterpret_cast<const uint4*>(row + off));
+    return v;
+}
+
+template <typename E>
+__device__ __forceinline__ uint4 few_load_edge(const char* row, int64_t off, int64_t n) {
+    if (off + 16 <= n) return __ldg(reinterpret_cast<const uint4*>(row + off));
+    alignas(16) E e[16 / sizeof(E)] = {};
+#pragma unroll
+    for (int i = 0; i < 16 / (int)sizeof(E); ++i)
+        if (off + (i + 1) * (int)sizeof(E) <= n) e[i] = reinterpret_cast<const E*>(row + off)[i];
+    return *reinterpret_cast<uint4*>(e);
+}
+
+template <bool GATE, typename E, int NT, typename O, int ACT>
+__global__ void __launch_bounds__(256, NT == 4 ? 2 : 3) k_few(const FewArgs a) {
+    constexpr bool kInt = sizeof(E) == 1;
+    constexpr int kRows = GATE ? 8 : 16;   // weight rows (channels) of a block
+    constexpr int kU = NT == 4 ? 2 : 4;    // 64-byte pieces of K in flight per warp
+    __shared__ uint32_t part[8][4 * NT][32];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+    const int n0 = blockIdx.x * kRows;
+    // rows and tokens beyond the last read the last one; their sums are not used
+    const char* r0 = a.w[0] + (int64_t)min(n0 + g, a.N - 1) * a.ldw[0] + t * 16;
+    const char* r1 = GATE ? a.w[1] + (int64_t)min(n0 + g, a.N - 1) * a.ldw[1] + t * 16
+                          : a.w[0] + (int64_t)min(n0 + g + 8, a.N - 1) * a.ldw[0] + t * 16;
+    const char* xr[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) xr[j] = a.x + (int64_t)min(j * 8 + g, a.T - 1) * a.ldx + t * 16;
+    uint32_t c[NT][4] = {};
+    auto multiply = [&](const uint4& w0, const uint4& w1, const uint4 (&x)[NT]) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            few_mma<kInt, E>(c[j], w0.x, w1.x, w0.y, w1.y, x[j].x, x[j].y);
+            few_mma<kInt, E>(c[j], w0.z, w1.z, w0.w, w1.w, x[j].z, x[j].w);
+        }
+    };
+    int64_t k = (int64_t)warp * kU * 64;
+    for (; k + kU * 64 <= a.kbytes; k += 8 * kU * 64) {
+        uint4 w0[kU], w1[kU], x[kU][NT];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            w0[u] = few_load<true>(r0, k + u * 64);
+            w1[u] = few_load<true>(r1, k + u * 64);
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) x[u][j] = few_load<false>(xr[j], k + u * 64);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) multiply(w0[u], w1[u], x[u]);
+    }
+    for (; k < a.kbytes; k += 64) {  // the piece that ends inside: one warp, once
+        const int64_t left = a.kbytes - t * 16;
+        const uint4 w0 = few_load_edge<E>(r0, k, left), w1 = few_load_edge<E>(r1, k, left);
+        uint4 x[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) x[j] = few_load_edge<E>(xr[j], k, left);
+        multiply(w0, w1, x);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[warp][j * 4 + i][lane] = c[j][i];
+    __syncthreads();
+    // element (token, channel pair): c[0..1] of a quad are tokens 2 t, 2 t + 1 of row g, c[2..3] those of row g + 8
+    for (int e = threadIdx.x; e < 64 * NT; e += 256) {
+        const int ch = e % 8, tok = e / 8;
+        const int from = ch * 4 + tok % 8 / 2, i = tok / 8 * 4 + tok % 2;
+        const int n = n0 + ch;
+        if constexpr (kInt) {
+            int s0 = 0, s1 = 0;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {
+                s0 += static_cast<int>(part[w][i][from]);
+                s1 += static_cast<int>(part[w][i + 2][from]);
+            }
+            const bool in0 = tok < a.T && n < a.N, in1 = tok < a.T && n + 8 < a.N;
+            const float rs = tok < a.T ? a.row_scale[tok] : 0.0f;
+            O* row = reinterpret_cast<O*>(a.c[0]) + tok * a.ld[0];
+            if (in0) row[n] = from_f32<O>(static_cast<float>(s0) * rs * a.col_scale[n]);
+            if (in1) row[n + 8] = from_f32<O>(static_cast<float>(s1) * rs * a.col_scale[n + 8]);
+            if (a.rowdiff) {
+                long long sum = (in0 ? (long long)s0 : 0) + (in1 ? (long long)s1 : 0);
+                for (int o = 4; o; o >>= 1) sum += __shfl_down_sync(~0u, sum, o, 8);
+                if (ch == 0 && tok < a.T) atomicAdd(a.rowdiff + tok, static_cast<unsigned long long>(sum));
+            }
+        } else {
+            float gate = 0.0f, up = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {
+                gate += __uint_as_float(part[w][i][from]);
+                up += __uint_as_float(part[w][i + 2][from]);
+            }
+            if (tok < a.T && n < a.N) {
+                reinterpret_cast<O*>(a.c[0])[tok * a.ld[0] + n] = from_f32<O>(act<ACT>(gate) * up);
+                if (a.c[1]) {
+                    reinterpret_cast<O*>(a.c[1])[tok * a.ld[1] + n] = from_f32<O>(gate);
+                    reinterpret_cast<O*>(a.c[2])[tok * a.ld[2] + n] = from_f32<O>(up);
+                }
+            }
+        }
+    }
+}
+
 __global__ void k_negate(const int64_t* __restrict__ in, int64_t* __restrict__ out, int n) {
     const int i = blockIdx.x * 256 + threadIdx.x;
     if (i < n) out[i] = -in[i];
@@ -484,17 +837,44 @@ __global__ void __launch_bounds__(256) k_pack(const T* __restrict__ in, int64_t 
         if (c < cols) out[r * ldo + c] = in[r * ld + c];
 }
 
-template <typename T, int ACT>
-__global__ void __launch_bounds__(256) k_gate_grad(const T* dh, int64_t ldd, const T* g, int64_t ldg, const T* u,
-                                                   int64_t ldu, int N, T* dg, T* du, int64_t ldo) {
-    const int n = blockIdx.y * 256 + threadIdx.x;
-    const int64_t t = blockIdx.x;
-    if (n >= N) return;
-    const float d = to_f32(dh[t * ldd + n]);
-    float a, slope;
-    act_grad<ACT>(to_f32(g[t * ldg + n]), a, slope);
-    dg[t * ldo + n] = from_f32<T>(d * to_f32(u[t * ldu + n]) * slope);
-    du[t * ldo + n] = from_f32<T>(d * a);
+// dgate = dh u act'(g), dup = dh act(g). Bound by its five matrices; 8 elements
+// per thread where every row is 16-byte aligned (VEC).
+struct GradArgs {
+    const void *dh, *g, *u;
+    int64_t ldd, ldg, ldu;
+    int T, N;
+    void *dg, *du;
+    int64_t ldo;
+};
+
+template <typename T, int ACT, bool VEC>
+__global__ void __launch_bounds__(256) k_gate_grad(const GradArgs a) {
+    const int pieces = (a.N + 7) / 8;
+    const int64_t count = (int64_t)a.T * pieces;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+        const int64_t t = i / pieces;
+        const int n = (int)(i - t * pieces) * 8;
+        Eight<T> d, g, u;
+        auto load = [&](Eight<T>& e, const void* p, int64_t ld) {
+            const T* row = reinterpret_cast<const T*>(p) + t * ld + n;
+            if (VEC && n + 8 <= a.N) e.load(row);
+            else e.load(row, a.N - n);
+        };
+        load(d, a.dh, a.ldd);
+        load(g, a.g, a.ldg);
+        load(u, a.u, a.ldu);
+        alignas(16) T og[8], ou[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float v, slope;
+            act_grad<ACT>(g[j], v, slope);
+            og[j] = from_f32<T>(d[j] * u[j] * slope);
+            ou[j] = from_f32<T>(d[j] * v);
+        }
+        // the pitch of dg and du holds whole pieces; what lies beyond N is not read by the products
+        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.dg) + t * a.ldo + n) = *reinterpret_cast<uint4*>(og);
+        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.du) + t * a.ldo + n) = *reinterpret_cast<uint4*>(ou);
+    }
 }
 
 // -------------------------------------------------------------------- host ---
@@ -562,6 +942,30 @@ int sm_count() {
     return n;
 }
 
+// Threads per row and pieces held by each: the smallest that hold a row of K.
+template <typename T>
+void quantize(const QuantArgs& a, cudaStream_t s) {
+    const bool vec = ((uintptr_t)a.x & 15) == 0 && (a.T == 1 || (a.ldx * (int64_t)sizeof(T) & 15) == 0) &&
+                     ((uintptr_t)a.q & 7) == 0 && (a.T == 1 || (a.ldq & 7) == 0) && ((uintptr_t)a.checksum & 15) == 0;
+    auto go = [&](auto row, auto u) {
+        constexpr int kRow = decltype(row)::value, kU = decltype(u)::value;
+        const unsigned grid = (unsigned)std::min<int64_t>(cdiv(a.T, 128 / kRow), (int64_t)sm_count() * 8);
+        if (vec)
+            k_quantize_rows<T, kRow, kU, true><<<grid, 128, 0, s>>>(a);
+        else
+            k_quantize_rows<T, kRow, kU, false><<<grid, 128, 0, s>>>(a);
+    };
+    using std::integral_constant;
+    const integral_constant<int, 32> warp;
+    const integral_constant<int, 128> block;
+    if (a.K <= 256) go(warp, integral_constant<int, 1>());
+    else if (a.K <= 1024) go(block, integral_constant<int, 1>());
+    else if (a.K <= 2048) go(block, integral_constant<int, 2>());
+    else if (a.K <= 4096) go(block, integral_constant<int, 4>());
+    else if (a.K <= 8192) go(block, integral_constant<int, 8>());
+    else go(block, integral_constant<int, 0>());
+}
+
 template <int MODE, int CG, int BN, typename O, int ACT>
 int launch_product(const Operand (&a)[2], const Operand (&b)[2], ProductArgs args, const char* name, cudaStream_t s) {
     using S = Shape<MODE, CG, BN>;
@@ -584,7 +988,13 @@ int launch_product(const Operand (&a)[2], const Operand (&b)[2], ProductArgs arg
     for (int i = 0; i < 3; ++i)
         args.wide[i] = ((uintptr_t)args.c[i] & 15) == 0 && (args.ld[i] * (int64_t)sizeof(O) & 15) == 0;
     auto kernel = k_product<MODE, CG, BN, O, ACT>;
-    cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    static std::atomic<uint64_t> ready{0};  // devices (of 64) on which the shared memory is allowed
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev > 63 || !(ready.load() >> dev & 1))) {
+        e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+        if (e == cudaSuccess && dev <= 63) ready.fetch_or(1ull << dev);
+    }
     if (e != cudaSuccess) return cuda_fail(e, name);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(std::min<int64_t>((int64_t)args.tiles_m * args.tiles_n, sm_count() / CG) * CG));
@@ -599,6 +1009,35 @@ int launch_product(const Operand (&a)[2], const Operand (&b)[2], ProductArgs arg
     cfg.numAttrs = 1;
     e = cudaLaunchKernelEx(&cfg, kernel, maps, args);
     return e == cudaSuccess ? ABFT_OK : cuda_fail(e, name);
+}
+
+constexpr int kFew = 32;  // tokens that k_few takes
+
+template <bool GATE, typename E, typename O, int ACT = 0>
+int few(const Operand& x, const Operand (&w)[2], const ProductArgs& p, const char* name, cudaStream_t s) {
+    FewArgs a = {};
+    for (int i = 0; i < 2; ++i) {
+        a.w[i] = (const char*)w[i].p;
+        a.ldw[i] = w[i].ld * w[i].size;
+    }
+    a.x = (const char*)x.p;
+    a.ldx = x.ld * x.size;
+    a.T = p.rows;
+    a.N = p.cols;
+    a.kbytes = (int64_t)x.cols * x.size;
+    std::copy(p.c, p.c + 3, a.c);
+    std::copy(p.ld, p.ld + 3, a.ld);
+    a.row_scale = p.row_scale;
+    a.col_scale = p.col_scale;
+    a.rowdiff = p.rowdiff;
+    const unsigned grid = (unsigned)cdiv(a.N, GATE ? 8 : 16);
+    if (a.T <= 8)
+        k_few<GATE, E, 1, O, ACT><<<grid, 256, 0, s>>>(a);
+    else if (a.T <= 16)
+        k_few<GATE, E, 2, O, ACT><<<grid, 256, 0, s>>>(a);
+    else
+        k_few<GATE, E, 4, O, ACT><<<grid, 256, 0, s>>>(a);
+    return launched(name);
 }
 
 // CTAs of one tile and columns of sums: pairs of SMs with the widest tile for
@@ -644,10 +1083,10 @@ int abft_quantize_rows(const void* dX, int64_t ldx, int type, int T, int K, int8
     if (T == 0) return ABFT_OK;
     if (!dX || !dQ || !dScale || (dChecksum != nullptr) != (dExpect != nullptr))
         return bad("abft_quantize_rows: bad argument (missing pointer, or one of dChecksum and dExpect alone)");
+    const QuantArgs args{dX, ldx, T, K, dQ, ldq, dScale, dChecksum, dExpect};
+    cudaStream_t s = (cudaStream_t)stream;
     auto go = [&](auto tag) {
-        using E = decltype(tag);
-        k_quantize_rows<E><<<T, 256, 0, (cudaStream_t)stream>>>((const E*)dX, ldx, K, dQ, ldq, dScale, dChecksum,
-                                                                dExpect);
+        quantize<decltype(tag)>(args, s);
         return launched("abft_quantize_rows");
     };
     if (type == ABFT_TYPE_F32) return go(0.0f);
@@ -657,7 +1096,14 @@ int abft_quantize_rows(const void* dX, int64_t ldx, int type, int T, int K, int8
 int abft_column_checksum(const int8_t* dW, int64_t ldw, int N, int K, int32_t* dChecksum, void* stream) {
     if (!dW || !dChecksum || N < 1 || N > ABFT_INT8_MAX_ROWS || K < 1 || ldw < K)
         return bad("abft_column_checksum: bad argument (need pointers, 1 <= N <= 2^24, K >= 1, ldw >= K)");
-    k_column_checksum<<<(unsigned)cdiv(K, 256), 256, 0, (cudaStream_t)stream>>>(dW, ldw, N, K, dChecksum);
+    cudaStream_t s = (cudaStream_t)stream;
+    const cudaError_t e = cudaMemsetAsync(dChecksum, 0, sizeof(int32_t) * K, s);
+    if (e != cudaSuccess) return cuda_fail(e, "abft_column_checksum");
+    const unsigned chunks = (unsigned)cdiv(N, 256);
+    if (((uintptr_t)dW & 3) == 0 && (ldw & 3) == 0)
+        k_column_checksum<true><<<dim3((unsigned)cdiv(K, 1024), chunks), 256, 0, s>>>(dW, ldw, N, K, dChecksum);
+    else
+        k_column_checksum<false><<<dim3((unsigned)cdiv(K, 256), chunks), 256, 0, s>>>(dW, ldw, N, K, dChecksum);
     return launched("abft_column_checksum");
 }
 
@@ -693,6 +1139,7 @@ int abft_int8_matmul(const int8_t* dQ, int64_t ldq, const float* dQScale, const 
     args.col_scale = dWScale;
     args.rowdiff = (unsigned long long*)dRowDiff;
     auto go = [&](auto tag) {
+        if (T <= kFew) return few<false, int8_t, decltype(tag)>(q, {w, w}, args, "abft_int8_matmul", s);
         return product<kInt8, decltype(tag)>({q, q}, {w, w}, args, "abft_int8_matmul", s);
     };
     if (type == ABFT_TYPE_F32) return go(0.0f);
@@ -735,6 +1182,8 @@ int abft_gated_ffn(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg
     std::copy(pitches, pitches + 3, args.ld);
     return with_type(type, [&](auto tag) {
         return with_act(activation, [&](auto a) {
+            if (T <= kFew)
+                return few<true, decltype(tag), decltype(tag), decltype(a)::value>(x, {wg, wu}, args, "abft_gated_ffn", s);
             return product<kGate, decltype(tag), decltype(a)::value>({x, x}, {wg, wu}, args, "abft_gated_ffn", s);
         });
     });
@@ -778,8 +1227,14 @@ int abft_gated_ffn_backward(const void* dDH, int64_t ldd, const void* dX, int64_
     return with_type(type, [&](auto tag) {
         using E = decltype(tag);
         with_act(activation, [&](auto a) {
-            k_gate_grad<E, decltype(a)::value><<<dim3(T, (unsigned)cdiv(N, 256)), 256, 0, s>>>(
-                (const E*)dDH, ldd, (const E*)dG, ldg, (const E*)dU, ldu, N, (E*)dg.p, (E*)du.p, p);
+            const GradArgs ga{dDH, dG, dU, ldd, ldg, ldu, T, N, const_cast<void*>(dg.p), const_cast<void*>(du.p), p};
+            const bool vec = Operand{dDH, ldd, T, N, 2}.direct() && Operand{dG, ldg, T, N, 2}.direct() &&
+                             Operand{dU, ldu, T, N, 2}.direct();
+            const unsigned grid = (unsigned)std::min<int64_t>(cdiv(T * cdiv(N, 8), 256), (int64_t)sm_count() * 64);
+            if (vec)
+                k_gate_grad<E, decltype(a)::value, true><<<grid, 256, 0, s>>>(ga);
+            else
+                k_gate_grad<E, decltype(a)::value, false><<<grid, 256, 0, s>>>(ga);
             return 0;
         });
         ProductArgs args = {};

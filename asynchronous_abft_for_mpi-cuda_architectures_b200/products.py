@@ -7,9 +7,11 @@ allocated on that stream; inputs handed to a stream that is not the current
 one are kept from reuse until its work is done. Nothing is kept between calls,
 so they can be captured into CUDA graphs and issued on several streams.
 """
+import contextlib
+
 import torch
 
-from ._lib import call, lib
+from ._lib import check, lib
 
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
@@ -20,7 +22,7 @@ INT8_MAX_ROWS = 1 << 24      # 127 * N fits a 32-bit checksum
 
 def _matrix(t, name, dtypes, rows=None, cols=None, device=None):
     """Checks a row-major CUDA matrix and returns its row pitch in elements."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.dtype in dtypes):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.ndim == 2 and t.dtype in dtypes):
         raise ValueError(f"{name} must be a 2-d CUDA tensor of {' or '.join(str(d)[6:] for d in dtypes)}")
     r, c = t.shape
     if (rows is not None and r != rows) or (cols is not None and c != cols):
@@ -53,33 +55,26 @@ def _activation(name):
     return ACTIVATIONS[name]
 
 
-class _On:
-    """The device and stream of one call."""
+_HERE = contextlib.nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
-    def __init__(self, device, stream, inputs):
-        self.device = device
-        self.guard = None
-        if stream is not None:
-            if not hasattr(stream, "cuda_stream"):
-                stream = torch.cuda.ExternalStream(int(stream), device=device)
-            if stream.device != device:
-                raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
-            if stream != torch.cuda.current_stream(device):
-                for t in inputs:
-                    if t is not None:
-                        t.record_stream(stream)
-            self.guard = torch.cuda.stream(stream)
-        elif device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(device)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _on(device, stream, inputs):
+    """(raw stream, context to allocate and launch in) of one call."""
+    if stream is None:
+        # the raw forms: torch.cuda.current_stream() alone is 2 us, as long as a launch
+        index = device.index
+        return _raw_stream(index), _HERE if index == _current_device() else torch.cuda.device(device)
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream), device=device)
+    if stream.device != device:
+        raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+    if stream != torch.cuda.current_stream(device):
+        for t in inputs:
+            if t is not None:
+                t.record_stream(stream)
+    return stream.cuda_stream, torch.cuda.stream(stream)
 
 
 def _work(nbytes, device):
@@ -92,12 +87,14 @@ def _ptr(t):
 
 def _empty8(rows, cols, device):
     """An 8-bit matrix on a pitch of 16 bytes."""
-    return torch.empty((rows, (cols + 15) & ~15), dtype=torch.int8, device=device)[:, :cols]
+    t = torch.empty((rows, (cols + 15) & ~15), dtype=torch.int8, device=device)
+    return t[:, :cols] if cols & 15 else t
 
 
 def _empty16(rows, cols, dtype, device):
     """A 16-bit matrix on a pitch of 16 bytes."""
-    return torch.empty((rows, (cols + 7) & ~7), dtype=dtype, device=device)[:, :cols]
+    t = torch.empty((rows, (cols + 7) & ~7), dtype=dtype, device=device)
+    return t[:, :cols] if cols & 7 else t
 
 
 def quantize_rows(x, checksum=None, stream=None):
@@ -113,17 +110,20 @@ def quantize_rows(x, checksum=None, stream=None):
     expect[t] = sum_k q[t, k] * checksum[k] (int64) is what int8_matmul's rows
     have to sum to.
     """
-    ldx = _matrix(x, "x", tuple(TYPES))
+    ldx = _matrix(x, "x", TYPES)
     T, K = x.shape
     dev = x.device
     if checksum is not None:
         _vector(checksum, "checksum", torch.int32, K, dev)
-    with _On(dev, stream, (x, checksum)) as s:
+    s, where = _on(dev, stream, (x, checksum))
+    with where:
         q = _empty8(T, K, dev)
         scale = torch.empty(T, dtype=torch.float32, device=dev)
         expect = None if checksum is None else torch.empty(T, dtype=torch.int64, device=dev)
-        call("abft_quantize_rows", x.data_ptr(), ldx, TYPES[x.dtype], T, K, q.data_ptr(), (K + 15) & ~15,
+        rc = lib.abft_quantize_rows(x.data_ptr(), ldx, TYPES[x.dtype], T, K, q.data_ptr(), (K + 15) & ~15,
              scale.data_ptr(), _ptr(checksum), _ptr(expect), s)
+        if rc:
+            check(rc, "abft_quantize_rows")
     return (q, scale) if checksum is None else (q, scale, expect)
 
 
@@ -133,9 +133,12 @@ def column_checksum(w, stream=None):
     N, K = w.shape
     if N < 1 or N > INT8_MAX_ROWS:
         raise ValueError(f"w has {N} rows: 1 to {INT8_MAX_ROWS} are supported")
-    with _On(w.device, stream, (w,)) as s:
+    s, where = _on(w.device, stream, (w,))
+    with where:
         out = torch.empty(K, dtype=torch.int32, device=w.device)
-        call("abft_column_checksum", w.data_ptr(), ldw, N, K, out.data_ptr(), s)
+        rc = lib.abft_column_checksum(w.data_ptr(), ldw, N, K, out.data_ptr(), s)
+        if rc:
+            check(rc, "abft_column_checksum")
     return out
 
 
@@ -163,14 +166,17 @@ def int8_matmul(q, q_scale, w, w_scale, dtype=torch.bfloat16, expect=None, strea
     _vector(w_scale, "w_scale", torch.float32, N, dev)
     if expect is not None:
         _vector(expect, "expect", torch.int64, T, dev)
-    with _On(dev, stream, (q, q_scale, w, w_scale, expect)) as s:
+    s, where = _on(dev, stream, (q, q_scale, w, w_scale, expect))
+    with where:
         y = torch.empty((T, N), dtype=dtype, device=dev)
         rowdiff = None if expect is None else torch.empty(T, dtype=torch.int64, device=dev)
         qp, wp = q.data_ptr(), w.data_ptr()
         nbytes = lib.abft_int8_matmul_ws_bytes(qp, ldq, wp, ldw, T, N, K)
         work = _work(nbytes, dev)
-        call("abft_int8_matmul", qp, ldq, q_scale.data_ptr(), wp, ldw, w_scale.data_ptr(), T, N, K, y.data_ptr(), N,
+        rc = lib.abft_int8_matmul(qp, ldq, q_scale.data_ptr(), wp, ldw, w_scale.data_ptr(), T, N, K, y.data_ptr(), N,
              TYPES[dtype], _ptr(expect), _ptr(rowdiff), _ptr(work), nbytes, s)
+        if rc:
+            check(rc, "abft_int8_matmul")
     return y if expect is None else (y, rowdiff)
 
 
@@ -198,7 +204,8 @@ def gated_ffn(x, w_gate, w_up, activation="silu", save=False, stream=None):
     ldx, ldwg, ldwu, T, N, K = _block(x, w_gate, w_up)
     act = _activation(activation)
     dev = x.device
-    with _On(dev, stream, (x, w_gate, w_up)) as s:
+    s, where = _on(dev, stream, (x, w_gate, w_up))
+    with where:
         h = _empty16(T, N, x.dtype, dev)
         g = _empty16(T, N, x.dtype, dev) if save else None
         u = _empty16(T, N, x.dtype, dev) if save else None
@@ -206,8 +213,10 @@ def gated_ffn(x, w_gate, w_up, activation="silu", save=False, stream=None):
         xp, gp, up = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr()
         nbytes = lib.abft_gated_ffn_ws_bytes(xp, ldx, gp, ldwg, up, ldwu, T, N, K)
         work = _work(nbytes, dev)
-        call("abft_gated_ffn", xp, ldx, gp, ldwg, up, ldwu, T, N, K, TYPES[x.dtype], act, h.data_ptr(), ld,
+        rc = lib.abft_gated_ffn(xp, ldx, gp, ldwg, up, ldwu, T, N, K, TYPES[x.dtype], act, h.data_ptr(), ld,
              _ptr(g), ld, _ptr(u), ld, _ptr(work), nbytes, s)
+        if rc:
+            check(rc, "abft_gated_ffn")
     return (h, g, u) if save else h
 
 
@@ -224,14 +233,17 @@ def gated_ffn_backward(dh, x, w_gate, w_up, g, u, activation="silu", stream=None
     ldd = _matrix(dh, "dh", same, T, N, dev)
     ldg = _matrix(g, "g", same, T, N, dev)
     ldu = _matrix(u, "u", same, T, N, dev)
-    with _On(dev, stream, (dh, x, w_gate, w_up, g, u)) as s:
+    s, where = _on(dev, stream, (dh, x, w_gate, w_up, g, u))
+    with where:
         dx = torch.empty((T, K), dtype=x.dtype, device=dev)
         dw_gate = torch.empty((N, K), dtype=x.dtype, device=dev)
         dw_up = torch.empty((N, K), dtype=x.dtype, device=dev)
         xp, gp, up = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr()
         nbytes = lib.abft_gated_ffn_backward_ws_bytes(xp, ldx, gp, ldwg, up, ldwu, T, N, K)
         work = _work(nbytes, dev)
-        call("abft_gated_ffn_backward", dh.data_ptr(), ldd, xp, ldx, gp, ldwg, up, ldwu, g.data_ptr(), ldg,
+        rc = lib.abft_gated_ffn_backward(dh.data_ptr(), ldd, xp, ldx, gp, ldwg, up, ldwu, g.data_ptr(), ldg,
              u.data_ptr(), ldu, T, N, K, TYPES[x.dtype], act, dx.data_ptr(), K, dw_gate.data_ptr(), K,
              dw_up.data_ptr(), K, _ptr(work), nbytes, s)
+        if rc:
+            check(rc, "abft_gated_ffn_backward")
     return dx, dw_gate, dw_up
