@@ -169,16 +169,23 @@ struct Eight {
     }
 };
 
-// 8 integers of a row in two words.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+    float m;
+    asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+    return m;
+}
+
+// kRound + the integers of 8 elements; the low bytes are the integers.
 template <typename T>
-__device__ __forceinline__ uint2 quantize_eight(const Eight<T>& e, float scale, float inv, float half, bool normal) {
-    float t[8];
+__device__ __forceinline__ void quantize_eight(const Eight<T>& e, float scale, float inv, float half, bool normal,
+                                               float (&t)[8]) {
     if (normal) {
         float worst = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 8; i += 2) {
             t[i] = fmaf(e[i], inv, kRound);
-            worst = fmaxf(worst, fabsf(fmaf(-(t[i] - kRound), scale, e[i])));
+            t[i + 1] = fmaf(e[i + 1], inv, kRound);
+            worst = max_abs(worst, fmaf(-(t[i] - kRound), scale, e[i]), fmaf(-(t[i + 1] - kRound), scale, e[i + 1]));
         }
         if (worst >= half) {
 #pragma unroll
@@ -188,25 +195,45 @@ __device__ __forceinline__ uint2 quantize_eight(const Eight<T>& e, float scale, 
 #pragma unroll
         for (int i = 0; i < 8; ++i) t[i] = kRound + static_cast<float>(quantize_tiny(e[i], scale));
     }
-    auto four = [&](int i) {
-        const uint32_t lo = __byte_perm(__float_as_uint(t[i]), __float_as_uint(t[i + 1]), 0x0040);
-        const uint32_t hi = __byte_perm(__float_as_uint(t[i + 2]), __float_as_uint(t[i + 3]), 0x0040);
-        return __byte_perm(lo, hi, 0x5410);
-    };
-    return make_uint2(four(0), four(4));
+}
+
+// Sum over a warp of 64-bit words that wrap: 27, 27 and 10 bits at a time, whose
+// sums over 32 lanes fit 32 bits.
+__device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
+    const uint32_t a = __reduce_add_sync(~0u, (uint32_t)v & 0x7ffffffu);
+    const uint32_t b = __reduce_add_sync(~0u, (uint32_t)(v >> 27) & 0x7ffffffu);
+    const uint32_t c = __reduce_add_sync(~0u, (uint32_t)(v >> 54));
+    return a + ((unsigned long long)b << 27) + ((unsigned long long)c << 54);
+}
+
+// Dot product of 4 signed and 4 unsigned bytes, added to c.
+__device__ __forceinline__ int dot_su(uint32_t a, int b, int c) {
+    int d;
+    asm("dp4a.s32.u32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+
+__device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
+    return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040),
+                       __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
 }
 
 // One row per group of ROW threads, U pieces of 8 elements per thread, held in
 // registers; U = 0: any number of pieces, read twice. VEC: rows of x and the
-// checksum are 16-byte and rows of q 8-byte aligned. Groups walk the rows, so that the checksum's
-// pieces are loaded once.
-template <typename T, int ROW, int U, bool VEC>
-__global__ void __launch_bounds__(128) k_quantize_rows(const QuantArgs a) {
+// checksum are 16-byte and rows of q 8-byte aligned. Groups walk the rows, the
+// next one loading while this one is rounded. With CHECK the checksum lies in
+// shared memory as its four bytes, the top one signed, four elements' in a word:
+// 4 of the 8-bit dot product instructions take 4 integers' share of the expected
+// sum (64-bit multiply-adds cost 3 instructions an element; 16384 rows of 4096
+// bfloat16: 55 us with them, 45 us so, 35 us without a checksum).
+template <typename T, int ROW, int U, bool VEC, bool CHECK>
+__global__ void __launch_bounds__(ROW < 128 ? 128 : ROW, 1024 / (ROW < 128 ? 128 : ROW))
+    k_quantize_rows(const QuantArgs a) {
     constexpr int kHeld = U > 0 ? U : 1;
-    constexpr bool kKeepSums = U > 0 && U <= 4;  // 8 registers of checksum a piece
-    __shared__ uint32_t smax[2][4];
-    __shared__ long long ssum[2][4];
-    const int me = threadIdx.x % ROW, groups = 128 / ROW;
+    constexpr int kBlock = ROW < 128 ? 128 : ROW, kGroups = kBlock / ROW, kWarps = ROW / 32;
+    __shared__ uint32_t smax[2][kWarps];
+    __shared__ unsigned long long ssum[2][kWarps];
+    const int me = threadIdx.x % ROW;
     const int pieces = (a.K + 7) / 8;
     auto load = [&](Eight<T>& e, const T* row, int p) {
         const int left = a.K - p * 8;
@@ -225,21 +252,52 @@ __global__ void __launch_bounds__(128) k_quantize_rows(const QuantArgs a) {
             for (int i = 0; i < 8; ++i) c[i] = p * 8 + i < a.K ? a.checksum[p * 8 + i] : 0;
         }
     };
-    int c[kKeepSums ? U : 1][8];
-    if (kKeepSums && a.checksum) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) checks(c[u], me + u * ROW);
+    extern __shared__ int4 bytes[];  // of all pieces' first halves, then of the second ones
+    if constexpr (CHECK && U > 0) {
+        auto transpose = [](const int* k) {
+            const uint32_t l01 = __byte_perm(k[0], k[1], 0x5140), h01 = __byte_perm(k[0], k[1], 0x7362);
+            const uint32_t l23 = __byte_perm(k[2], k[3], 0x5140), h23 = __byte_perm(k[2], k[3], 0x7362);
+            return make_int4(__byte_perm(l01, l23, 0x5410), __byte_perm(l01, l23, 0x7632),
+                             __byte_perm(h01, h23, 0x5410), __byte_perm(h01, h23, 0x7632));
+        };
+        for (int p = threadIdx.x; p < pieces; p += kBlock) {
+            int k[8];
+            checks(k, p);
+            bytes[p] = transpose(k);
+            bytes[pieces + p] = transpose(k + 4);
+        }
+        __syncthreads();
     }
     int flip = 0;
-    for (int64_t row = (int64_t)blockIdx.x * groups + threadIdx.x / ROW; row < a.T;
-         row += (int64_t)gridDim.x * groups, flip ^= 1) {
+    int64_t last = -1;  // the row whose warps' sums lie in shared memory
+    auto finish = [&](int f) {
+        if (me != 0 || last < 0) return;
+        unsigned long long sum = 0;
+        for (int w = 0; w < kWarps; ++w) sum += ssum[f][w];
+        a.expect[last] = (int64_t)sum;
+    };
+    const int64_t first = (int64_t)blockIdx.x * kGroups + threadIdx.x / ROW, stride = (int64_t)gridDim.x * kGroups;
+    constexpr bool kAhead = U > 0 && sizeof(T) == 2;  // 32-bit rows would not fit the registers twice
+    Eight<T> e[kHeld], next[kAhead ? kHeld : 1];
+    auto fetch = [&](Eight<T>* to, int64_t row) {
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) load(to[u], reinterpret_cast<const T*>(a.x) + row * a.ldx, me + u * ROW);
+    };
+    if constexpr (kAhead)
+        if (first < a.T) fetch(next, first);
+    for (int64_t row = first; row < a.T; row += stride, flip ^= 1) {
         const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx;
         int8_t* q = a.q + row * a.ldq;
-        Eight<T> e[kHeld];
         uint32_t m = 0;
         if constexpr (U > 0) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) load(e[u], x, me + u * ROW);
+            for (int u = 0; u < U; ++u)
+                if constexpr (kAhead) e[u] = next[u];
+            if constexpr (kAhead) {
+                if (row + stride < a.T) fetch(next, row + stride);
+            } else {
+                fetch(e, row);
+            }
 #pragma unroll
             for (int u = 0; u < U; ++u) m = e[u].largest(m);
         } else {
@@ -251,58 +309,75 @@ __global__ void __launch_bounds__(128) k_quantize_rows(const QuantArgs a) {
             }
         }
         m = __reduce_max_sync(~0u, Eight<T>::magnitude(m));
-        if constexpr (ROW == 128) {
+        if constexpr (kWarps > 1) {
             if (threadIdx.x % 32 == 0) smax[flip][threadIdx.x / 32] = m;
             __syncthreads();
-            m = max(max(smax[flip][0], smax[flip][1]), max(smax[flip][2], smax[flip][3]));
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) m = max(m, smax[flip][w]);
+            if constexpr (CHECK) finish(flip ^ 1);  // of the row before, by this row's barrier
         }
         const bool finite = m < 0x7f800000u;
         const float s = finite ? __fdiv_rn(__uint_as_float(m), 127.0f) : __uint_as_float(0x7fc00000u);
         const bool normal = s >= 0x1p-100f;
-        const float inv = 1.0f / s, half = 0.5f * s;
-        long long sum = 0;
-        auto write = [&](const Eight<T>& v, int p, const int (&k)[8]) {
+        const float inv = __fdiv_rn(1.0f, s), half = 0.5f * s;
+        int dot[4] = {};              // below 2^31: at most 32 integers of 127 times 255
+        unsigned long long sum = 0;   // U = 0: K is not bounded
+        auto write = [&](const Eight<T>& v, int p) {
             const int left = a.K - p * 8;
             if (left <= 0) return;
-            const uint2 w = quantize_eight(v, s, inv, half, normal);
+            float t[8];
+            quantize_eight(v, s, inv, half, normal, t);
+            const uint32_t lo = low_bytes(t[0], t[1], t[2], t[3]), hi = low_bytes(t[4], t[5], t[6], t[7]);
             if (VEC && left >= 8) {
-                *reinterpret_cast<uint2*>(q + p * 8) = w;
+                *reinterpret_cast<uint2*>(q + p * 8) = make_uint2(lo, hi);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (i < left) q[p * 8 + i] = static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+                    if (i < left) q[p * 8 + i] = static_cast<int8_t>((i < 4 ? lo : hi) >> (8 * (i & 3)));
             }
-            if (a.checksum) {
+            if constexpr (CHECK && U > 0) {
+                const int4 first = bytes[p], second = bytes[pieces + p];
+                dot[0] = dot_su(lo, first.x, dot_su(hi, second.x, dot[0]));
+                dot[1] = dot_su(lo, first.y, dot_su(hi, second.y, dot[1]));
+                dot[2] = dot_su(lo, first.z, dot_su(hi, second.z, dot[2]));
+                dot[3] = __dp4a((int)lo, first.w, __dp4a((int)hi, second.w, dot[3]));
+            } else if constexpr (CHECK) {
+                int k[8];
+                checks(k, p);
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    sum += (long long)static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3))) * k[i];
+                    sum += (unsigned long long)((long long)static_cast<int8_t>(__float_as_int(t[i])) * k[i]);
             }
         };
         if constexpr (U > 0) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if constexpr (!kKeepSums)
-                    if (a.checksum) checks(c[0], me + u * ROW);
-                write(e[u], me + u * ROW, c[kKeepSums ? u : 0]);
-            }
+            for (int u = 0; u < U; ++u) write(e[u], me + u * ROW);
         } else {
+#pragma unroll 2
             for (int p = me; p < pieces; p += ROW) {
                 load(e[0], x, p);
-                if (a.checksum) checks(c[0], p);
-                write(e[0], p, c[0]);
+                write(e[0], p);
             }
         }
         if (me == 0) a.scale[row] = s;
-        if (a.checksum) {
-#pragma unroll
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-            if constexpr (ROW == 128) {
-                if (threadIdx.x % 32 == 0) ssum[flip][threadIdx.x / 32] = sum;
-                __syncthreads();
-                sum = ssum[flip][0] + ssum[flip][1] + ssum[flip][2] + ssum[flip][3];
+        if constexpr (CHECK) {
+            if constexpr (U > 0) {
+                for (int i = 3; i >= 0; --i)
+                    sum = sum * 256 + (unsigned long long)(long long)__reduce_add_sync(~0u, dot[i]);
+            } else {
+                sum = warp_sum(sum);
             }
-            if (me == 0) a.expect[row] = sum;
+            if constexpr (kWarps > 1) {
+                if (threadIdx.x % 32 == 0) ssum[flip][threadIdx.x / 32] = sum;
+                last = row;
+            } else if (me == 0) {
+                a.expect[row] = (int64_t)sum;
+            }
         }
+    }
+    if constexpr (CHECK && kWarps > 1) {
+        __syncthreads();
+        finish(flip ^ 1);
     }
 }
 
@@ -942,28 +1017,49 @@ int sm_count() {
     return n;
 }
 
-// Threads per row and pieces held by each: the smallest that hold a row of K.
+// Threads per row and pieces held by each: the smallest that hold a row of K;
+// a warp alone needs no barrier. Unaligned rows are walked.
 template <typename T>
 void quantize(const QuantArgs& a, cudaStream_t s) {
     const bool vec = ((uintptr_t)a.x & 15) == 0 && (a.T == 1 || (a.ldx * (int64_t)sizeof(T) & 15) == 0) &&
                      ((uintptr_t)a.q & 7) == 0 && (a.T == 1 || (a.ldq & 7) == 0) && ((uintptr_t)a.checksum & 15) == 0;
-    auto go = [&](auto row, auto u) {
-        constexpr int kRow = decltype(row)::value, kU = decltype(u)::value;
-        const unsigned grid = (unsigned)std::min<int64_t>(cdiv(a.T, 128 / kRow), (int64_t)sm_count() * 8);
-        if (vec)
-            k_quantize_rows<T, kRow, kU, true><<<grid, 128, 0, s>>>(a);
-        else
-            k_quantize_rows<T, kRow, kU, false><<<grid, 128, 0, s>>>(a);
-    };
     using std::integral_constant;
+    auto launch = [&](auto row, auto u, auto v, auto check) {
+        constexpr int kRow = decltype(row)::value, kU = decltype(u)::value, kBlock = kRow < 128 ? 128 : kRow;
+        // as many blocks as are resident at a time
+        const int smem = decltype(check)::value && kU > 0 ? (int)cdiv(a.K, 8) * 32 : 0;
+        auto kernel = k_quantize_rows<T, kRow, kU, decltype(v)::value, decltype(check)::value>;
+        if (smem > 48 * 1024) (void)cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
+        int64_t blocks = cdiv(a.T, kBlock / kRow);
+        if (blocks > sm_count()) {  // as many as are resident at a time, each with the same number of rows
+            int resident = 1;
+            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kBlock, smem) != cudaSuccess) resident = 1;
+            blocks = std::min<int64_t>(blocks, (int64_t)sm_count() * resident);
+        }
+        kernel<<<(unsigned)blocks, kBlock, smem, s>>>(a);
+    };
+    const std::true_type yes;
+    const std::false_type no;
     const integral_constant<int, 32> warp;
-    const integral_constant<int, 128> block;
-    if (a.K <= 256) go(warp, integral_constant<int, 1>());
-    else if (a.K <= 1024) go(block, integral_constant<int, 1>());
-    else if (a.K <= 2048) go(block, integral_constant<int, 2>());
-    else if (a.K <= 4096) go(block, integral_constant<int, 4>());
-    else if (a.K <= 8192) go(block, integral_constant<int, 8>());
-    else go(block, integral_constant<int, 0>());
+    const integral_constant<int, 128> row128;
+    const integral_constant<int, 256> row256;
+    const integral_constant<int, 512> row512;
+    const integral_constant<int, 0> walk;
+    const integral_constant<int, 1> one;
+    const integral_constant<int, 2> two;
+    const integral_constant<int, 4> four;
+    auto choose = [&](auto check) {
+        if (!vec) a.K <= 1024 ? launch(warp, walk, no, check) : launch(row256, walk, no, check);
+        else if (a.K <= 256) launch(warp, one, yes, check);
+        else if (a.K <= 512) launch(warp, two, yes, check);
+        else if (a.K <= 1024) launch(warp, four, yes, check);
+        else if (a.K <= 2048) launch(row128, two, yes, check);
+        else if (a.K <= 4096) launch(row128, four, yes, check);
+        else if (a.K <= 8192) launch(row256, four, yes, check);
+        else if (a.K <= 16384) launch(row512, four, yes, check);
+        else launch(row512, walk, yes, check);
+    };
+    a.checksum ? choose(yes) : choose(no);
 }
 
 template <int MODE, int CG, int BN, typename O, int ACT>
