@@ -420,12 +420,19 @@ __global__ void __launch_bounds__(256) k_column_checksum(const int8_t* __restric
 //   kDw     dg^T x and du^T x                  A: dg or du       B: x, both MN-major
 //
 // Warp 0 copies operand tiles to shared memory (TMA, 128-byte swizzle), one
-// thread of warp 1 issues the matrix instructions, warps 4-7 take finished
+// thread of warp 1 issues the matrix instructions, warps 4-11 take finished
 // sums out of tensor memory; sums are double-buffered there, so the next
 // tile's products run while this one is written. With CG = 2 two CTAs (two
 // SMs) form one 256-row tile: each holds its 128 rows of A and half of B, and
 // the matrix instruction of the leader reads both halves, which halves the
 // copies of B per product.
+//
+// Finished sums go through a small piece of shared memory, so that a warp
+// writes whole 64- or 128-byte runs of each output row, aligned or not.
+//
+// SPLIT: when there are too few tiles for the GPU, the CTAs of a cluster share
+// one tile's K; their partial sums meet in shared memory (each CTA adds up its
+// share of the rows in a fixed order, reading the others' over the cluster).
 //
 // Nothing is transposed in memory: an operand whose summed index runs along
 // the pitch is MN-major, which the matrix instructions read directly. Rows and
@@ -439,6 +446,7 @@ struct ProductArgs {
     int tiles_m, tiles_n;        // kDw: tiles_m counts both outputs' tiles
     int tiles_m1;                // of the first output
     int chunks;                  // of 128 bytes along K, one operand pair
+    int split;                   // CTAs that share a tile's K
     int limit;                   // polls of a wait
     void* c[3];                  // outputs; kGate: h, g, u; kDw: dWg, dWu
     int64_t ld[3];
@@ -455,21 +463,26 @@ struct ProductMaps {
 // Waits that ran out since the last abft_products_status, any product kernel of the device.
 __device__ unsigned g_fault;
 
-template <int MODE, int CG, int BN>
+constexpr int kProductThreads = 384;  // copies, matrix instructions, 2 idle warps (one holds tensor memory), 8 for results
+
+template <int MODE, int CG, int BN, typename O>
 struct Shape {
     static constexpr bool kTwoPairs = MODE == kDx;
     static constexpr bool kAMn = MODE == kDw;
     static constexpr bool kBMn = MODE == kDx || MODE == kDw;
-    static constexpr int kARows = 128;                 // per CTA
-    static constexpr int kBRows = BN / CG;             // per CTA
-    static constexpr int kStageBytes = (kARows + kBRows) * 128;
-    static constexpr int kStages = (BN == 256 && CG == 1) ? 4 : (BN <= 64 ? 8 : 6);
-    static constexpr int kStagesEnd = kStages * kStageBytes;
-    static constexpr int kBars = kStagesEnd + 4 * 256 * 4;  // after the epilogue warps' scales
+    static constexpr int kCols = MODE == kGate ? BN / 2 : BN;  // of an output
+    static constexpr int kABytes = 128 * 128, kBBytes = BN / CG * 128;  // of a stage, per CTA
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kOutBytes = 32 * (32 * (int)sizeof(O) + 16);  // 32 x 32 results on their way out, one warp
+    // 227 KB of shared memory: alignment, barriers, 8 warps' results and channel scales; the rest are stages
+    static constexpr int kRoom = 227 * 1024 - 1024 - 512 - 8 * kOutBytes - 8 * 128 * 4;
+    static constexpr int kStages = kRoom / kStageBytes < 8 ? kRoom / kStageBytes : 8;
+    static constexpr int kOut = kStages * kStageBytes;
+    static constexpr int kScales = kOut + 8 * kOutBytes;
+    static constexpr int kBars = kScales + 8 * 128 * 4;
     static constexpr int kSmem = 1024 + kBars + 512;
-    static constexpr int kOutCols = MODE == kGate ? BN / 2 : BN;
     static constexpr int kTmemCols = 2 * BN;
-    };
+};
 
 // A wait with a limit. `stop` is set for the whole CTA by the first that runs out.
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, int limit, volatile int* stop) {
@@ -484,42 +497,54 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, int limi
     return false;
 }
 
-// Tile order: groups of 8 tile rows, columns inside a group, so that the CTAs
-// at work at one time read few operand rows (L2 hits).
+// Tile order: groups of 16 tile rows, columns inside a group, so that the CTAs
+// at work at one time read few operand rows (L2 hits). 8192 x 16384 x 4096
+// block: 1680 us with groups of 8, 1640 of 16, 1710 of 32.
 __device__ __forceinline__ void tile_at(int i, int tiles_m, int tiles_n, int& m, int& n) {
-    const int group = 8 * tiles_n;
+    const int group = 16 * tiles_n;
     const int g = i / group, r = i - g * group;
-    const int h = min(8, tiles_m - g * 8);
+    const int h = min(16, tiles_m - g * 16);
     n = r / h;
-    m = g * 8 + r - n * h;
+    m = g * 16 + r - n * h;
 }
 
-// 32 values to row `row` of a matrix from column n on.
+// A warp's 32 x 32 values (one row per lane) to a matrix at `to`, of which
+// `rows` rows and `cols` columns exist; `wide`: 16-byte stores are possible.
 template <typename O>
-__device__ __forceinline__ void store32(O* row, int n, int cols, bool wide, const float (&v)[32]) {
-    constexpr int kV = 16 / sizeof(O);
+__device__ __forceinline__ void store_block(char* mine, O* to, int64_t ld, int rows, int cols, bool wide,
+                                            const float (&v)[32]) {
+    constexpr int kV = 16 / sizeof(O), kPieces = 32 / kV, kPitch = 32 * sizeof(O) + 16;
+    const int lane = threadIdx.x % 32;
+    __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 32; j += kV) {
-        if (wide && n + j + kV <= cols) {
-            alignas(16) O pack[kV];
+    for (int j = 0; j < kPieces; ++j) {
+        alignas(16) O pack[kV];
 #pragma unroll
-            for (int i = 0; i < kV; ++i) pack[i] = from_f32<O>(v[j + i]);
-            *reinterpret_cast<uint4*>(row + n + j) = *reinterpret_cast<uint4*>(pack);
-        } else {
+        for (int i = 0; i < kV; ++i) pack[i] = from_f32<O>(v[j * kV + i]);
+        *reinterpret_cast<uint4*>(mine + lane * kPitch + j * 16) = *reinterpret_cast<uint4*>(pack);
+    }
+    __syncwarp();
+    if (wide && cols >= 32) {
+        const int r = lane / kPieces, piece = lane % kPieces;
 #pragma unroll
-            for (int i = 0; i < kV; ++i)
-                if (n + j + i < cols) row[n + j + i] = from_f32<O>(v[j + i]);
-        }
+        for (int i = 0; i < 32; i += 32 / kPieces)
+            if (i + r < rows)
+                *reinterpret_cast<uint4*>(to + (i + r) * ld + piece * kV) =
+                    *reinterpret_cast<uint4*>(mine + (i + r) * kPitch + piece * 16);
+    } else if (lane < cols) {
+        for (int i = 0; i < 32 && i < rows; ++i)
+            to[i * ld + lane] = *reinterpret_cast<O*>(mine + i * kPitch + lane * sizeof(O));
     }
 }
 
-template <int MODE, int CG, int BN, typename O, int ACT>
-__global__ void __launch_bounds__(256, 1) k_product(const __grid_constant__ ProductMaps maps, const ProductArgs a) {
-    using S = Shape<MODE, CG, BN>;
+template <int MODE, int CG, int BN, bool SPLIT, typename O, int ACT>
+__global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_constant__ ProductMaps maps, const ProductArgs a) {
+    using S = Shape<MODE, CG, BN, O>;
+    constexpr int kPart = BN + 4;  // SPLIT: pitch of the partial sums, which overlay the stages
+    static_assert(!SPLIT || CG == 1, "a split tile is one CTA wide");
     extern __shared__ char raw[];
     char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const uint32_t base = tensor::smem_u32(smem);
-    float* scales = reinterpret_cast<float*>(smem + S::kStagesEnd);
     const uint32_t bars = base + S::kBars;
     auto full = [&](int s) { return bars + 8 * s; };
     auto empty = [&](int s) { return bars + 8 * (S::kStages + s); };
@@ -529,11 +554,16 @@ __global__ void __launch_bounds__(256, 1) k_product(const __grid_constant__ Prod
     volatile int* stop = reinterpret_cast<volatile int*>(smem + S::kBars + 8 * (2 * S::kStages + 5));
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(const_cast<int*>(stop) + 1);
 
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t rank = CG == 2 ? tensor::cluster_rank() : 0;
+    // the same in all lanes, and known to be
+    const int warp = __shfl_sync(~0u, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+    const uint32_t in_cluster = CG == 2 || SPLIT ? tensor::cluster_rank() : 0;
+    const uint32_t rank = SPLIT ? 0 : in_cluster;  // in the pair
     const int tiles = a.tiles_m * a.tiles_n;
-    const int first = blockIdx.x / CG, step = gridDim.x / CG;
-    const int chunks = S::kTwoPairs ? 2 * a.chunks : a.chunks;
+    const int first = SPLIT ? blockIdx.x / a.split : blockIdx.x / CG, step = SPLIT ? tiles : gridDim.x / CG;
+    const int all = S::kTwoPairs ? 2 * a.chunks : a.chunks;
+    // this CTA's part of K
+    const int begin = SPLIT ? (int)((int64_t)all * in_cluster / a.split) : 0;
+    const int end = SPLIT ? (int)((int64_t)all * (in_cluster + 1) / a.split) : all;
     constexpr int kElems = MODE == kInt8 ? 128 : 64;  // of 128 bytes along K
 
     if (threadIdx.x == 0) {
@@ -543,7 +573,7 @@ __global__ void __launch_bounds__(256, 1) k_product(const __grid_constant__ Prod
         }
         for (int s = 0; s < 2; ++s) {
             tensor::bar_init(sums_full(s), 1);
-            tensor::bar_init(sums_empty(s), 4 * CG);
+            tensor::bar_init(sums_empty(s), 8 * CG);
         }
         tensor::bar_init(drained, 1);
         *stop = 0;
@@ -556,13 +586,19 @@ __global__ void __launch_bounds__(256, 1) k_product(const __grid_constant__ Prod
     tensor::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0 && lane == 0) {
+    // The stages go round: `s` is the stage, `turn` the parity of its round. Both
+    // loops below run in one elected thread and keep every address in a counter:
+    // with divisions by the number of stages, and a vote of the warp per wait,
+    // their own instructions took 0.21 us a chunk.
+    if (warp == 0 && tensor::elect()) {
         // ------------------------------------------------ copies ---
         for (int i = 0; i < 2; ++i) {
             tensor::prefetch_map(&maps.a[i]);
             tensor::prefetch_map(&maps.b[i]);
         }
-        int it = 0;
+        const uint32_t done0 = CG == 2 ? tensor::in_leader(full(0)) : full(0);
+        int s = 0, issued = 0;
+        uint32_t turn = 0;
         bool ok = true;
         for (int tile = first; ok && tile < tiles; tile += step) {
             int mt, nt;
@@ -573,16 +609,15 @@ __global__ void __launch_bounds__(256, 1) k_product(const __grid_constant__ Prod
                 pair = 1;
             }
             const int m0 = (mt * CG + (int)rank) * 128;
-            const int n0 = MODE == kGate ? nt * S::kOutCols : nt * BN + (int)rank * S::kBRows;
-            for (int c = 0; c < chunks; ++c, ++it) {
-                const int s = it % S::kStages;
-                if (!wait_for(empty(s), (it / S::kStages + 1) & 1, a.limit, stop)) {
+            const int n0 = nt * S::kCols;
+            for (int c = begin; c < end; ++c) {
+                if (!wait_for(empty(s), turn ^ 1, a.limit, stop)) {
                     ok = false;
                     break;
                 }
                 if (rank == 0) tensor::bar_expect(full(s), CG * S::kStageBytes);
-                const uint32_t done = CG == 2 ? tensor::in_leader(full(s)) : full(s);
-                const uint32_t sa = base + s * S::kStageBytes, sb = sa + S::kARows * 128;
+                const uint32_t done = done0 + 8 * s;
+                const uint32_t sa = base + s * S::kStageBytes;
                 int k = c;
                 if constexpr (S::kTwoPairs) {
                     pair = c >= a.chunks;
@@ -595,59 +630,74 @@ __global__ void __launch_bounds__(256, 1) k_product(const __grid_constant__ Prod
                 } else {
                     tensor::tma_load<CG>(sa, am, k * kElems, m0, done);
                 }
+                const uint32_t sb = sa + S::kABytes;
                 if constexpr (S::kBMn) {
                     const CUtensorMap* bm = MODE == kDx ? &maps.b[pair] : &maps.b[0];
 #pragma unroll
-                    for (int j = 0; j < S::kBRows / 64; ++j)
-                        tensor::tma_load<CG>(sb + j * 8192, bm, n0 + j * 64, k * 64, done);
+                    for (int j = 0; j < BN / CG / 64; ++j)
+                        tensor::tma_load<CG>(sb + j * 8192, bm, n0 + (int)rank * (BN / CG) + j * 64, k * 64, done);
                 } else if constexpr (MODE == kGate && CG == 2) {
                     tensor::tma_load<CG>(sb, &maps.b[rank], k * kElems, n0, done);
                 } else if constexpr (MODE == kGate) {
                     tensor::tma_load<CG>(sb, &maps.b[0], k * kElems, n0, done);
-                    tensor::tma_load<CG>(sb + BN / 2 * 128, &maps.b[1], k * kElems, n0, done);
+                    tensor::tma_load<CG>(sb + S::kBBytes / 2, &maps.b[1], k * kElems, n0, done);
                 } else {
-                    tensor::tma_load<CG>(sb, &maps.b[0], k * kElems, n0, done);
+                    tensor::tma_load<CG>(sb, &maps.b[0], k * kElems, n0 + (int)rank * (BN / CG), done);
+                }
+                issued = min(issued + 1, S::kStages);
+                if (++s == S::kStages) {
+                    s = 0;
+                    turn ^= 1;
                 }
             }
         }
-        // The CTA stays until the last stages are read (the pair's leader signals both CTAs).
-        for (int j = max(0, it - S::kStages); ok && j < it; ++j)
-            ok = wait_for(empty(j % S::kStages), (j / S::kStages) & 1, a.limit, stop);
+        // The CTA stays until its last stages are read (the pair's leader signals both CTAs).
+        auto last = [&](auto&& wait) {
+            for (int j = 0, t = s, r = turn; j < issued; ++j) {
+                if (--t < 0) {
+                    t = S::kStages - 1;
+                    r ^= 1;
+                }
+                wait(t, r);
+            }
+        };
+        last([&](int t, int r) { ok = ok && wait_for(empty(t), r, a.limit, stop); });
         if (!ok) {  // after a wait that ran out the copies in flight land first
             if (rank == 0)
-                for (int j = max(0, it - S::kStages); j < it; ++j)
-                    for (int i = 0; i < kWaitLimit && !tensor::bar_test(full(j % S::kStages), (j / S::kStages) & 1); ++i) {
+                last([&](int t, int r) {
+                    for (int i = 0; i < kWaitLimit && !tensor::bar_test(full(t), r); ++i) {
                     }
+                });
             else
-                for (int i = 0; i < 1000 && it > 0; ++i) __nanosleep(1000);
+                for (int i = 0; i < 1000 && issued > 0; ++i) __nanosleep(1000);
         }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1 && tensor::elect()) {
         // ------------------------------------- matrix instructions ---
-        constexpr uint32_t idesc =
-            tensor::instruction(128 * CG, BN, MODE == kInt8, std::is_same<O, __nv_bfloat16>::value, S::kAMn, S::kBMn);
+        constexpr uint32_t idesc = tensor::instruction(128 * CG, BN, MODE == kInt8, std::is_same<O, __nv_bfloat16>::value,
+                                                       S::kAMn, S::kBMn);
         constexpr uint32_t a_step = S::kAMn ? 2048 >> 4 : 32 >> 4, b_step = S::kBMn ? 2048 >> 4 : 32 >> 4;
-        int it = 0, n = 0;
+        const uint64_t a0 = tensor::operand(base, S::kAMn), b0 = tensor::operand(base + S::kABytes, S::kBMn);
+        int s = 0, n = 0;
+        uint32_t turn = 0;
         bool ok = true;
         for (int tile = first; rank == 0 && ok && tile < tiles; tile += step, ++n) {
-            const int buf = n & 1;
-            if (!wait_for(sums_empty(buf), ((n >> 1) + 1) & 1, a.limit, stop)) break;
-            tensor::tc_fence_after();
-            const uint32_t d = tmem + buf * BN;
-            for (int c = 0; c < chunks; ++c, ++it) {
-                const int s = it % S::kStages;
-                if (!wait_for(full(s), (it / S::kStages) & 1, a.limit, stop)) {
-                    ok = false;
-                    break;
-                }
+            ok = wait_for(sums_empty(n & 1), ((n >> 1) + 1) & 1, a.limit, stop);
+            const uint32_t d = tmem + (n & 1) * BN;
+            for (int c = begin; ok && c < end; ++c) {
+                ok = wait_for(full(s), turn, a.limit, stop);
+                if (!ok) break;
                 tensor::tc_fence_after();
-                const uint32_t sa = base + s * S::kStageBytes;
-                const uint64_t da = tensor::operand(sa, S::kAMn), db = tensor::operand(sa + S::kARows * 128, S::kBMn);
+                const uint64_t da = a0 + s * (S::kStageBytes >> 4), db = b0 + s * (S::kStageBytes >> 4);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    tensor::mma<CG, MODE == kInt8>(d, da + k * a_step, db + k * b_step, idesc, c > 0 || k > 0);
+                    tensor::mma<CG, MODE == kInt8>(d, da + k * a_step, db + k * b_step, idesc, c > begin || k > 0);
                 tensor::mma_commit<CG>(empty(s));
+                if (++s == S::kStages) {
+                    s = 0;
+                    turn ^= 1;
+                }
             }
-            if (ok) tensor::mma_commit<CG>(sums_full(buf));
+            if (ok) tensor::mma_commit<CG>(sums_full(n & 1));
         }
         // instructions in flight still read shared and write tensor memory, in both CTAs of a pair
         if (rank == 0) tensor::mma_commit<CG>(drained);
@@ -655,8 +705,13 @@ __global__ void __launch_bounds__(256, 1) k_product(const __grid_constant__ Prod
         }
     } else if (warp >= 4) {
         // -------------------------------------------------- results ---
-        const int w = warp - 4;
+        // warps w and w + 4 take the same 32 rows, each half of the columns
+        const int w = warp % 4, half = warp / 8;
+        constexpr int kBlocks = (SPLIT ? BN : S::kCols) / 32;
+        const int j0 = half ? (kBlocks + 1) / 2 * 32 : 0, j1 = half ? kBlocks * 32 : (kBlocks + 1) / 2 * 32;
         const uint32_t lanes = tmem + ((uint32_t)w << 21);
+        char* mine = smem + S::kOut + (warp - 4) * S::kOutBytes;
+        float* sc = reinterpret_cast<float*>(smem + S::kScales) + (warp - 4) * 128;
         int n = 0;
         for (int tile = first; tile < tiles; tile += step, ++n) {
             const int buf = n & 1;
@@ -667,75 +722,167 @@ __global__ void __launch_bounds__(256, 1) k_product(const __grid_constant__ Prod
                 mt -= a.tiles_m1;
                 out = 1;
             }
-            const int m = (mt * CG + (int)rank) * 128 + w * 32 + lane;
-            const int n0 = nt * S::kOutCols;
-            const bool live = m < a.rows;
-            float* sc = scales + w * 256;
+            const int m0 = (mt * CG + (int)rank) * 128 + w * 32;  // the warp's first row
+            const int rows = a.rows - m0;
+            const int n0 = nt * S::kCols;
+            long long total = 0;
             float rs = 0.0f;
-            if constexpr (MODE == kInt8) {
+            if constexpr (MODE == kInt8 && !SPLIT) {
+                if (lane < rows) rs = a.row_scale[m0 + lane];
                 __syncwarp();
-                for (int j = lane; j < BN; j += 32) sc[j] = n0 + j < a.cols ? a.col_scale[n0 + j] : 0.0f;
-                if (live) rs = a.row_scale[m];
+                for (int j = j0 + lane; j < j1; j += 32) sc[j - j0] = n0 + j < a.cols ? a.col_scale[n0 + j] : 0.0f;
                 __syncwarp();
             }
             if (!__all_sync(~0u, wait_for(sums_full(buf), (n >> 1) & 1, a.limit, stop))) break;
             tensor::tc_fence_after();
-            long long total = 0;
+            auto put = [&](int i, int j, const float(&v)[32]) {
+                store_block<O>(mine, reinterpret_cast<O*>(a.c[i]) + m0 * a.ld[i] + n0 + j, a.ld[i], rows,
+                               a.cols - n0 - j, a.wide[i], v);
+            };
+            auto taken = [&] {  // the sums are out: the next tile may overwrite them
+                tensor::tc_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    tensor::bar_arrive_cluster(CG == 2 ? tensor::in_leader(sums_empty(buf)) : sums_empty(buf));
+            };
+            if (!SPLIT && j0 == j1) taken();
 #pragma unroll 1
-            for (int j = 0; j < S::kOutCols; j += 32) {
+            for (int j = j0; j < j1; j += 32) {
                 uint32_t r[32], r2[32];
                 __syncwarp();
                 tensor::tmem_load32(lanes + buf * BN + j, r);
-                if constexpr (MODE == kGate) tensor::tmem_load32(lanes + buf * BN + BN / 2 + j, r2);
+                if constexpr (MODE == kGate && !SPLIT) tensor::tmem_load32(lanes + buf * BN + S::kCols + j, r2);
                 tensor::tmem_wait_load(r);
-                if constexpr (MODE == kGate) tensor::after_wait(r2);
-                if (j + 32 == S::kOutCols) {  // the sums are out: the next tile may overwrite them
-                    tensor::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0)
-                        tensor::bar_arrive_cluster(CG == 2 ? tensor::in_leader(sums_empty(buf)) : sums_empty(buf));
-                }
-                if (live) {
-                    float v[32];
-                    if constexpr (MODE == kInt8) {
-    #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int sum = static_cast<int>(r[i]);
-                            total += sum;
-                            v[i] = static_cast<float>(sum) * rs * sc[j + i];
-                        }
-                        store32<O>(reinterpret_cast<O*>(a.c[0]) + m * a.ld[0], n0 + j, a.cols, a.wide[0], v);
-                    } else if constexpr (MODE == kGate) {
-                        float u[32];
-    #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            v[i] = __uint_as_float(r[i]);
-                            u[i] = __uint_as_float(r2[i]);
-                        }
-                        if (a.c[1]) {
-                            store32<O>(reinterpret_cast<O*>(a.c[1]) + m * a.ld[1], n0 + j, a.cols, a.wide[1], v);
-                            store32<O>(reinterpret_cast<O*>(a.c[2]) + m * a.ld[2], n0 + j, a.cols, a.wide[2], u);
-                        }
-    #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = act<ACT>(v[i]) * u[i];
-                        store32<O>(reinterpret_cast<O*>(a.c[0]) + m * a.ld[0], n0 + j, a.cols, a.wide[0], v);
-                    } else {
-    #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-                        store32<O>(reinterpret_cast<O*>(a.c[out]) + m * a.ld[out], n0 + j, a.cols, a.wide[out], v);
+                if constexpr (MODE == kGate && !SPLIT) tensor::after_wait(r2);
+                if (!SPLIT && j + 32 == j1) taken();
+                float v[32];
+                if constexpr (SPLIT) {
+                    uint4* part = reinterpret_cast<uint4*>(smem + ((w * 32 + lane) * kPart + j) * 4);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) part[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+                } else if constexpr (MODE == kInt8) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int sum = static_cast<int>(r[i]);
+                        total += sum;
+                        v[i] = static_cast<float>(sum) * rs * sc[j - j0 + i];
                     }
+                    put(0, j, v);
+                } else if constexpr (MODE == kGate) {
+                    float up[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        v[i] = __uint_as_float(r[i]);
+                        up[i] = __uint_as_float(r2[i]);
+                    }
+                    if (a.c[1]) {
+                        put(1, j, v);
+                        put(2, j, up);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = act<ACT>(v[i]) * up[i];
+                    put(0, j, v);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+                    put(out, j, v);
                 }
             }
-            if (MODE == kInt8 && live && a.rowdiff)
-                atomicAdd(a.rowdiff + m, static_cast<unsigned long long>(total));
+            // sums of columns and rows beyond the matrices are zeros
+            if (MODE == kInt8 && !SPLIT && lane < rows && a.rowdiff)
+                atomicAdd(a.rowdiff + m0 + lane, static_cast<unsigned long long>(total));
         }
     }
     __syncwarp();
     tensor::tc_fence_before();
     __syncthreads();
-    if constexpr (CG == 2) tensor::cluster_sync();
+    if constexpr (CG == 2 || SPLIT) tensor::cluster_sync();
     tensor::tc_fence_after();
     if (warp == 2) tensor::tmem_free<CG>(tmem, S::kTmemCols);
+
+    if constexpr (SPLIT) {
+        // every CTA adds up its share of the tile's rows: a thread takes 4 columns of a row, all CTAs' parts of them at once
+        int mt, nt;
+        tile_at(first, a.tiles_m, a.tiles_n, mt, nt);
+        int out = 0;
+        if (MODE == kDw && mt >= a.tiles_m1) {
+            mt -= a.tiles_m1;
+            out = 1;
+        }
+        constexpr int kFours = S::kCols / 4;  // threads of a row, 32 at most
+        const int n0 = nt * S::kCols, share = 128 / a.split;
+        auto sum = [&](int r, int c, auto(&v)[4]) {
+            uint4 part[8];
+#pragma unroll
+            for (int p = 0; p < 8; ++p)
+                if (p < a.split) part[p] = tensor::load_from(base + (r * kPart + c) * 4, p);
+#pragma unroll
+            for (int p = 0; p < 8; ++p)
+                if (p < a.split) {
+                    const uint32_t q[4] = {part[p].x, part[p].y, part[p].z, part[p].w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (MODE == kInt8) v[i] += static_cast<int>(q[i]);
+                        else v[i] += __uint_as_float(q[i]);
+                    }
+                }
+        };
+        auto put = [&](int i, int64_t m, int c, const float(&v)[4]) {
+            O* to = reinterpret_cast<O*>(a.c[i]) + m * a.ld[i] + n0 + c;
+            if (a.wide[i] && n0 + c + 4 <= a.cols) {
+                alignas(16) O pack[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) pack[j] = from_f32<O>(v[j]);
+                if constexpr (sizeof(O) == 4) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<uint4*>(pack);
+                else *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(pack);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (n0 + c + j < a.cols) to[j] = from_f32<O>(v[j]);
+            }
+        };
+        // whole warps go round together: share * kFours is a multiple of 32
+        for (int e = threadIdx.x; e < share * kFours; e += kProductThreads) {
+            const int r = (int)in_cluster * share + e / kFours, c = e % kFours * 4;
+            const int64_t m = mt * 128 + r;
+            const bool live = m < a.rows;
+            if constexpr (MODE == kInt8) {
+                int v[4] = {};
+                sum(r, c, v);
+                float y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    y[i] = static_cast<float>(v[i]) * (live ? a.row_scale[m] : 0.0f) *
+                           (n0 + c + i < a.cols ? a.col_scale[n0 + c + i] : 0.0f);
+                if (live) put(0, m, c, y);
+                if (a.rowdiff) {
+                    long long total = (long long)v[0] + v[1] + v[2] + v[3];
+#pragma unroll
+                    for (int o = kFours / 2; o; o >>= 1) total += __shfl_down_sync(~0u, total, o, kFours);
+                    if (c == 0 && live) atomicAdd(a.rowdiff + m, static_cast<unsigned long long>(total));
+                }
+            } else if constexpr (MODE == kGate) {
+                float g[4] = {}, up[4] = {};
+                sum(r, c, g);
+                sum(r, c + S::kCols, up);
+                if (live) {
+                    if (a.c[1]) {
+                        put(1, m, c, g);
+                        put(2, m, c, up);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) g[i] = act<ACT>(g[i]) * up[i];
+                    put(0, m, c, g);
+                }
+            } else {
+                float v[4] = {};
+                sum(r, c, v);
+                if (live) put(out, m, c, v);
+            }
+        }
+        __syncwarp();
+        tensor::cluster_sync();  // the others still read this CTA's sums
+    }
 }
 
 // ------------------------------------------------------------ few tokens ---
@@ -1062,11 +1209,11 @@ void quantize(const QuantArgs& a, cudaStream_t s) {
     a.checksum ? choose(yes) : choose(no);
 }
 
-template <int MODE, int CG, int BN, typename O, int ACT>
+template <int MODE, int CG, int BN, bool SPLIT, typename O, int ACT>
 int launch_product(const Operand (&a)[2], const Operand (&b)[2], ProductArgs args, const char* name, cudaStream_t s) {
-    using S = Shape<MODE, CG, BN>;
+    using S = Shape<MODE, CG, BN, O>;
     ProductMaps maps;
-    const int b_box = S::kBMn ? 64 : MODE == kGate ? BN / 2 : S::kBRows;
+    const int b_box = S::kBMn ? 64 : MODE == kGate ? BN / 2 : BN / CG;
     const int a_box = S::kAMn ? 64 : 128;
     bool made = a[0].map(&maps.a[0], a_box) && b[0].map(&maps.b[0], b_box);
     maps.a[1] = maps.a[0];
@@ -1079,11 +1226,11 @@ int launch_product(const Operand (&a)[2], const Operand (&b)[2], ProductArgs arg
     }
     args.tiles_m1 = (int)cdiv(args.rows, 128 * CG);
     args.tiles_m = MODE == kDw ? 2 * args.tiles_m1 : args.tiles_m1;
-    args.tiles_n = (int)cdiv(args.cols, S::kOutCols);
+    args.tiles_n = (int)cdiv(args.cols, S::kCols);
     args.limit = wait_limit();
     for (int i = 0; i < 3; ++i)
         args.wide[i] = ((uintptr_t)args.c[i] & 15) == 0 && (args.ld[i] * (int64_t)sizeof(O) & 15) == 0;
-    auto kernel = k_product<MODE, CG, BN, O, ACT>;
+    auto kernel = k_product<MODE, CG, BN, SPLIT, O, ACT>;
     static std::atomic<uint64_t> ready{0};  // devices (of 64) on which the shared memory is allowed
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -1092,14 +1239,15 @@ int launch_product(const Operand (&a)[2], const Operand (&b)[2], ProductArgs arg
         if (e == cudaSuccess && dev <= 63) ready.fetch_or(1ull << dev);
     }
     if (e != cudaSuccess) return cuda_fail(e, name);
+    const int64_t tiles = (int64_t)args.tiles_m * args.tiles_n;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(std::min<int64_t>((int64_t)args.tiles_m * args.tiles_n, sm_count() / CG) * CG));
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3((unsigned)(SPLIT ? tiles * args.split : std::min<int64_t>(tiles, sm_count() / CG) * CG));
+    cfg.blockDim = dim3(kProductThreads);
     cfg.dynamicSmemBytes = S::kSmem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.x = SPLIT ? args.split : CG;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
@@ -1136,16 +1284,54 @@ int few(const Operand& x, const Operand (&w)[2], const ProductArgs& p, const cha
     return launched(name);
 }
 
-// CTAs of one tile and columns of sums: pairs of SMs with the widest tile for
-// enough tiles to fill the GPU, single ones with narrower tiles below that.
+// Tile and split by an estimate in us: a start and an end that grow with the
+// tile, and for every round of tiles its chunks of 128 bytes of K, a chunk
+// costing what it does on a busy GPU:
+//
+//                       start + end   a chunk   (measured alone / all SMs busy)
+//   pair of SMs, 256        7.0        0.31      0.28 / 0.34
+//   one SM, 128 columns     5.0        0.21      0.18 / 0.24
+//   one SM, 64 columns      4.4        0.19      0.17 / 0.22
+//   split, 128 columns      7.2        0.20      for all CTAs at once only
+//   split, 64 columns       6.7        0.19
+//
+// Examples, bf16 block, us measured (256 / 128 / 64 / best split): 8192 x 16384 x
+// 4096 1540 / 2288 / - / -; 512 x 4096 x 4096 27 / 34 / 53 / 56; 2048 x 1536 x 1024
+// 16.7 / 15.7 / 23.9 / 49; 128 x 1536 x 1024 11.0 / 7.7 / 7.3 / 8.3; 128 x 4096 x 4096
+// 24.9 / 17.5 / 16.6 / 14.3; 128 x 1024 x 4096 24.3 / 16.7 / 15.9 / 10.3. Clusters of 8
+// do not fill the GPU (13 us where 4 take 8), so they stay at 64 CTAs.
 template <int MODE, typename O, int ACT = 0>
-int product(const Operand (&a)[2], const Operand (&b)[2], const ProductArgs& args, const char* name, cudaStream_t s) {
-    const int64_t outputs = MODE == kDw ? 2 : 1, width = MODE == kGate ? 2 : 1;
-    const int64_t rows = outputs * cdiv(args.rows, 128);
-    if (outputs * cdiv(args.rows, 256) * cdiv(args.cols * width, 256) >= 4)
-        return launch_product<MODE, 2, 256, O, ACT>(a, b, args, name, s);
-    if (rows * cdiv(args.cols * width, 128) >= 2) return launch_product<MODE, 1, 128, O, ACT>(a, b, args, name, s);
-    return launch_product<MODE, 1, 64, O, ACT>(a, b, args, name, s);
+int product(const Operand (&a)[2], const Operand (&b)[2], ProductArgs args, const char* name, cudaStream_t s) {
+    const int chunks = args.chunks * (MODE == kDx ? 2 : 1);
+    auto tiles = [&](int rows, int columns) {
+        return (MODE == kDw ? 2 : 1) * cdiv(args.rows, rows) * cdiv(args.cols, MODE == kGate ? columns / 2 : columns);
+    };
+    const int sms = sm_count();
+    double best = 1e30;
+    int which = 0;
+    auto consider = [&](int i, int split, double ends, double chunk, int64_t rounds) {
+        const double us = ends + chunk * (double)rounds * (double)cdiv(chunks, split);
+        if (us < best) {
+            best = us;
+            which = i;
+            args.split = split;
+        }
+    };
+    consider(0, 1, 7.0, 0.31, cdiv(tiles(256, 256), std::max(sms / 2, 1)));
+    consider(1, 1, 5.0, 0.21, cdiv(tiles(128, 128), sms));
+    consider(2, 1, 4.4, 0.19, cdiv(tiles(128, 64), sms));
+    for (int split = 2; split <= 8 && split <= chunks; split *= 2) {
+        const int most = split == 8 ? 64 : std::min(sms, 128);
+        if (tiles(128, 128) * split <= most) consider(3, split, 7.2, 0.20, 1);
+        if (tiles(128, 64) * split <= most) consider(4, split, 6.7, 0.19, 1);
+    }
+    switch (which) {
+        case 0: return launch_product<MODE, 2, 256, false, O, ACT>(a, b, args, name, s);
+        case 1: return launch_product<MODE, 1, 128, false, O, ACT>(a, b, args, name, s);
+        case 2: return launch_product<MODE, 1, 64, false, O, ACT>(a, b, args, name, s);
+        case 3: return launch_product<MODE, 1, 128, true, O, ACT>(a, b, args, name, s);
+        default: return launch_product<MODE, 1, 64, true, O, ACT>(a, b, args, name, s);
+    }
 }
 
 // dgate | dup, each T rows on a pitch of 16 bytes
