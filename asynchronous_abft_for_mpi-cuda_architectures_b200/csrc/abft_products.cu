@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 #include <type_traits>
 
@@ -107,7 +108,37 @@ __device__ __noinline__ int quantize_tiny(float x, float scale) {
     return static_cast<int>(fminf(fmaxf(t - kRound, -127.0f), 127.0f));
 }
 
+// 16 bytes at any address inside [begin, end): two aligned loads and a shift, or,
+// where those would leave the range, element by element.
+template <typename T>
+__device__ __forceinline__ uint4 load_any(const T* at, const void* begin, const void* end) {
+    const char* p = reinterpret_cast<const char*>(at);
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
+    const char* low = p - off;
+    if (off == 0) return __ldg(reinterpret_cast<const uint4*>(p));
+    if (low < begin || low + 32 > end) {
+        alignas(16) T e[16 / sizeof(T)];
+#pragma unroll
+        for (int i = 0; i < 16 / (int)sizeof(T); ++i) e[i] = at[i];
+        return *reinterpret_cast<uint4*>(e);
+    }
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(low)), b = __ldg(reinterpret_cast<const uint4*>(low) + 1);
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (off & 8) {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (off & 4) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    const int bits = (off & 3) * 8;
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                      __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
 struct QuantArgs {
+    bool aligned;    // rows of x and the checksum to 16 bytes, rows of q to 8
     const void* x;
     int64_t ldx;
     int T, K;
@@ -126,6 +157,10 @@ struct Eight {
     __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    }
+    __device__ __forceinline__ void load_any(const T* p, const void* begin, const void* end) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = abft::load_any<T>(p + i * (16 / sizeof(T)), begin, end);
     }
     __device__ __forceinline__ void load(const T* p, int n) {  // n of them, zeros after
         alignas(16) T e[8] = {};
@@ -219,14 +254,13 @@ __device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d
 }
 
 // One row per group of ROW threads, U pieces of 8 elements per thread, held in
-// registers; U = 0: any number of pieces, read twice. VEC: rows of x and the
-// checksum are 16-byte and rows of q 8-byte aligned. Groups walk the rows, the
+// registers; U = 0: any number of pieces, read twice. Groups walk the rows, the
 // next one loading while this one is rounded. With CHECK the checksum lies in
 // shared memory as its four bytes, the top one signed, four elements' in a word:
 // 4 of the 8-bit dot product instructions take 4 integers' share of the expected
 // sum (64-bit multiply-adds cost 3 instructions an element; 16384 rows of 4096
 // bfloat16: 55 us with them, 45 us so, 35 us without a checksum).
-template <typename T, int ROW, int U, bool VEC, bool CHECK>
+template <typename T, int ROW, int U, bool CHECK>
 __global__ void __launch_bounds__(ROW < 128 ? 128 : ROW, 1024 / (ROW < 128 ? 128 : ROW))
     k_quantize_rows(const QuantArgs a) {
     constexpr int kHeld = U > 0 ? U : 1;
@@ -235,14 +269,20 @@ __global__ void __launch_bounds__(ROW < 128 ? 128 : ROW, 1024 / (ROW < 128 ? 128
     __shared__ unsigned long long ssum[2][kWarps];
     const int me = threadIdx.x % ROW;
     const int pieces = (a.K + 7) / 8;
+    const T* x_end = reinterpret_cast<const T*>(a.x) + (a.T - 1) * a.ldx + a.K;
     auto load = [&](Eight<T>& e, const T* row, int p) {
         const int left = a.K - p * 8;
-        if (VEC && left >= 8) e.load(row + p * 8);
-        else if (left > 0) e.load(row + p * 8, left);
-        else e.zero();
+        if (left >= 8) {
+            if (a.aligned) e.load(row + p * 8);
+            else e.load_any(row + p * 8, a.x, x_end);
+        } else if (left > 0) {
+            e.load(row + p * 8, left);
+        } else {
+            e.zero();
+        }
     };
     auto checks = [&](int (&c)[8], int p) {
-        if (VEC && p * 8 + 8 <= a.K) {
+        if (a.aligned && p * 8 + 8 <= a.K) {
             const int4 lo = __ldg(reinterpret_cast<const int4*>(a.checksum + p * 8));
             const int4 hi = __ldg(reinterpret_cast<const int4*>(a.checksum + p * 8) + 1);
             c[0] = lo.x, c[1] = lo.y, c[2] = lo.z, c[3] = lo.w;
@@ -252,6 +292,17 @@ __global__ void __launch_bounds__(ROW < 128 ? 128 : ROW, 1024 / (ROW < 128 ? 128
             for (int i = 0; i < 8; ++i) c[i] = p * 8 + i < a.K ? a.checksum[p * 8 + i] : 0;
         }
     };
+    tensor::wait_for_stream();
+    tensor::let_next_start();
+    const int64_t first = (int64_t)blockIdx.x * kGroups + threadIdx.x / ROW, stride = (int64_t)gridDim.x * kGroups;
+    constexpr bool kAhead = U > 0 && sizeof(T) == 2;  // 32-bit rows would not fit the registers twice
+    Eight<T> e[kHeld], next[kAhead ? kHeld : 1];
+    auto fetch = [&](Eight<T>* to, int64_t row) {
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) load(to[u], reinterpret_cast<const T*>(a.x) + row * a.ldx, me + u * ROW);
+    };
+    if constexpr (kAhead)
+        if (first < a.T) fetch(next, first);
     extern __shared__ int4 bytes[];  // of all pieces' first halves, then of the second ones
     if constexpr (CHECK && U > 0) {
         auto transpose = [](const int* k) {
@@ -276,15 +327,6 @@ __global__ void __launch_bounds__(ROW < 128 ? 128 : ROW, 1024 / (ROW < 128 ? 128
         for (int w = 0; w < kWarps; ++w) sum += ssum[f][w];
         a.expect[last] = (int64_t)sum;
     };
-    const int64_t first = (int64_t)blockIdx.x * kGroups + threadIdx.x / ROW, stride = (int64_t)gridDim.x * kGroups;
-    constexpr bool kAhead = U > 0 && sizeof(T) == 2;  // 32-bit rows would not fit the registers twice
-    Eight<T> e[kHeld], next[kAhead ? kHeld : 1];
-    auto fetch = [&](Eight<T>* to, int64_t row) {
-#pragma unroll
-        for (int u = 0; u < kHeld; ++u) load(to[u], reinterpret_cast<const T*>(a.x) + row * a.ldx, me + u * ROW);
-    };
-    if constexpr (kAhead)
-        if (first < a.T) fetch(next, first);
     for (int64_t row = first; row < a.T; row += stride, flip ^= 1) {
         const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx;
         int8_t* q = a.q + row * a.ldq;
@@ -328,7 +370,7 @@ __global__ void __launch_bounds__(ROW < 128 ? 128 : ROW, 1024 / (ROW < 128 ? 128
             float t[8];
             quantize_eight(v, s, inv, half, normal, t);
             const uint32_t lo = low_bytes(t[0], t[1], t[2], t[3]), hi = low_bytes(t[4], t[5], t[6], t[7]);
-            if (VEC && left >= 8) {
+            if (a.aligned && left >= 8) {
                 *reinterpret_cast<uint2*>(q + p * 8) = make_uint2(lo, hi);
             } else {
 #pragma unroll
@@ -585,6 +627,8 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
     if constexpr (CG == 2) tensor::cluster_sync();
     tensor::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    tensor::wait_for_stream();
+    tensor::let_next_start();
 
     // The stages go round: `s` is the stage, `turn` the parity of its round. Both
     // loops below run in one elected thread and keep every address in a counter:
@@ -887,10 +931,10 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
 
 // ------------------------------------------------------------ few tokens ---
 //
-// Products of at most 32 tokens are bound by reading the weight once. The
+// Products of few tokens are bound by reading the weight once. The
 // 128-row tiles of the kernel above would leave most SMs without a tile and the
-// rest waiting on few copies, so here each block takes 16 weight rows (kGate: 8
-// of either weight) over all of K and its 8 warps share K: a warp reads 64 bytes
+// rest waiting on few copies, so here a group of WK warps takes 16 weight rows
+// (kGate: 8 of either weight) and shares their K: a warp reads runs of 64 bytes
 // of 16 rows with 16-byte loads straight into the registers of the 16 x 8
 // matrix instruction (weights are its 16 rows, tokens its 8 columns). The sum
 // over K does not depend on the order of K, so lane t of a quad simply takes
@@ -954,14 +998,14 @@ __device__ __forceinline__ uint4 few_load_edge(const char* row, int64_t off, int
     return *reinterpret_cast<uint4*>(e);
 }
 
-template <bool GATE, typename E, int NT, typename O, int ACT>
-__global__ void __launch_bounds__(256, NT == 4 ? 2 : 3) k_few(const FewArgs a) {
+template <bool GATE, typename E, int NT, int WK, typename O, int ACT>
+__global__ void __launch_bounds__(256, 2) k_few(const FewArgs a) {
     constexpr bool kInt = sizeof(E) == 1;
-    constexpr int kRows = GATE ? 8 : 16;   // weight rows (channels) of a block
-    constexpr int kU = NT == 4 ? 2 : 4;    // 64-byte pieces of K in flight per warp
+    constexpr int kRows = GATE ? 8 : 16;   // weight rows (channels) of a group of WK warps
+    constexpr int kU = NT == 4 ? 4 : 8;    // 64-byte pieces of K in flight per warp
     __shared__ uint32_t part[8][4 * NT][32];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-    const int n0 = blockIdx.x * kRows;
+    const int n0 = (blockIdx.x * (8 / WK) + warp / WK) * kRows;
     // rows and tokens beyond the last read the last one; their sums are not used
     const char* r0 = a.w[0] + (int64_t)min(n0 + g, a.N - 1) * a.ldw[0] + t * 16;
     const char* r1 = GATE ? a.w[1] + (int64_t)min(n0 + g, a.N - 1) * a.ldw[1] + t * 16
@@ -977,22 +1021,25 @@ __global__ void __launch_bounds__(256, NT == 4 ? 2 : 3) k_few(const FewArgs a) {
             few_mma<kInt, E>(c[j], w0.z, w1.z, w0.w, w1.w, x[j].z, x[j].w);
         }
     };
-    int64_t k = (int64_t)warp * kU * 64;
-    for (; k + kU * 64 <= a.kbytes; k += 8 * kU * 64) {
-        uint4 w0[kU], w1[kU], x[kU][NT];
+    tensor::wait_for_stream();
+    tensor::let_next_start();
+    int64_t k = (int64_t)(warp % WK) * kU * 64;
+    for (; k + kU * 64 <= a.kbytes; k += WK * kU * 64) {
+        uint4 w0[kU], w1[kU];
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             w0[u] = few_load<true>(r0, k + u * 64);
             w1[u] = few_load<true>(r1, k + u * 64);
         }
 #pragma unroll
-        for (int u = 0; u < kU; ++u)
+        for (int u = 0; u < kU; ++u) {
+            uint4 x[NT];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) x[u][j] = few_load<false>(xr[j], k + u * 64);
-#pragma unroll
-        for (int u = 0; u < kU; ++u) multiply(w0[u], w1[u], x[u]);
+            for (int j = 0; j < NT; ++j) x[j] = few_load<false>(xr[j], k + u * 64);
+            multiply(w0[u], w1[u], x);
+        }
     }
-    for (; k < a.kbytes; k += 64) {  // the piece that ends inside: one warp, once
+    for (; k < a.kbytes; k += 64) {  // the pieces of the run that ends inside: one warp of the group, once
         const int64_t left = a.kbytes - t * 16;
         const uint4 w0 = few_load_edge<E>(r0, k, left), w1 = few_load_edge<E>(r1, k, left);
         uint4 x[NT];
@@ -1006,16 +1053,16 @@ __global__ void __launch_bounds__(256, NT == 4 ? 2 : 3) k_few(const FewArgs a) {
         for (int i = 0; i < 4; ++i) part[warp][j * 4 + i][lane] = c[j][i];
     __syncthreads();
     // element (token, channel pair): c[0..1] of a quad are tokens 2 t, 2 t + 1 of row g, c[2..3] those of row g + 8
-    for (int e = threadIdx.x; e < 64 * NT; e += 256) {
-        const int ch = e % 8, tok = e / 8;
+    for (int e = threadIdx.x; e < 64 * NT * (8 / WK); e += 256) {
+        const int ch = e % 8, tok = e / 8 % (8 * NT), first = e / (64 * NT) * WK;
         const int from = ch * 4 + tok % 8 / 2, i = tok / 8 * 4 + tok % 2;
-        const int n = n0 + ch;
+        const int n = (blockIdx.x * (8 / WK) + first / WK) * kRows + ch;
         if constexpr (kInt) {
             int s0 = 0, s1 = 0;
 #pragma unroll
-            for (int w = 0; w < 8; ++w) {
-                s0 += static_cast<int>(part[w][i][from]);
-                s1 += static_cast<int>(part[w][i + 2][from]);
+            for (int w = 0; w < WK; ++w) {
+                s0 += static_cast<int>(part[first + w][i][from]);
+                s1 += static_cast<int>(part[first + w][i + 2][from]);
             }
             const bool in0 = tok < a.T && n < a.N, in1 = tok < a.T && n + 8 < a.N;
             const float rs = tok < a.T ? a.row_scale[tok] : 0.0f;
@@ -1030,9 +1077,9 @@ __global__ void __launch_bounds__(256, NT == 4 ? 2 : 3) k_few(const FewArgs a) {
         } else {
             float gate = 0.0f, up = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 8; ++w) {
-                gate += __uint_as_float(part[w][i][from]);
-                up += __uint_as_float(part[w][i + 2][from]);
+            for (int w = 0; w < WK; ++w) {
+                gate += __uint_as_float(part[first + w][i][from]);
+                up += __uint_as_float(part[first + w][i + 2][from]);
             }
             if (tok < a.T && n < a.N) {
                 reinterpret_cast<O*>(a.c[0])[tok * a.ld[0] + n] = from_f32<O>(act<ACT>(gate) * up);
@@ -1045,18 +1092,42 @@ __global__ void __launch_bounds__(256, NT == 4 ? 2 : 3) k_few(const FewArgs a) {
     }
 }
 
-__global__ void k_negate(const int64_t* __restrict__ in, int64_t* __restrict__ out, int n) {
+__global__ void __launch_bounds__(256) k_negate(const int64_t* __restrict__ in, int64_t* __restrict__ out, int n) {
+    tensor::wait_for_stream();
+    tensor::let_next_start();
     const int i = blockIdx.x * 256 + threadIdx.x;
     if (i < n) out[i] = -in[i];
 }
 
-// Copies rows onto a pitch of 16 bytes.
+// Rows of up to three matrices onto a pitch of 16 bytes, 16 bytes a thread.
+struct PackArgs {
+    const char* in[3];
+    char* out[3];
+    int64_t ld[3];       // bytes
+    int64_t row[3];      // bytes of a row
+    int64_t chunks[3];   // of 16 bytes of a row's copy
+    int64_t end[3];      // chunks of this matrix and those before it
+    int rows[3];
+};
+
 template <typename T>
-__global__ void __launch_bounds__(256) k_pack(const T* __restrict__ in, int64_t ld, int rows, int cols, T* __restrict__ out,
-                                              int64_t ldo) {
-    const int c = blockIdx.y * 256 + threadIdx.x;
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
-        if (c < cols) out[r * ldo + c] = in[r * ld + c];
+__global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
+    tensor::wait_for_stream();
+    tensor::let_next_start();
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.end[2]; i += (int64_t)gridDim.x * 256) {
+        const int m = i < a.end[0] ? 0 : i < a.end[1] ? 1 : 2;
+        const int64_t e = i - (m == 0 ? 0 : a.end[m - 1]), r = e / a.chunks[m], c = (e - r * a.chunks[m]) * 16;
+        const char* row = a.in[m] + r * a.ld[m];
+        uint4 v;
+        if (c + 16 <= a.row[m]) {
+            v = load_any(reinterpret_cast<const T*>(row + c), a.in[m], a.in[m] + (a.rows[m] - 1) * a.ld[m] + a.row[m]);
+        } else {
+            alignas(16) T last[16 / sizeof(T)] = {};
+            for (int j = 0; c + j * (int)sizeof(T) < a.row[m]; ++j) last[j] = reinterpret_cast<const T*>(row + c)[j];
+            v = *reinterpret_cast<uint4*>(last);
+        }
+        *reinterpret_cast<uint4*>(a.out[m] + r * a.chunks[m] * 16 + c) = v;
+    }
 }
 
 // dgate = dh u act'(g), dup = dh act(g). Bound by its five matrices; 8 elements
@@ -1071,6 +1142,8 @@ struct GradArgs {
 
 template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(256) k_gate_grad(const GradArgs a) {
+    tensor::wait_for_stream();
+    tensor::let_next_start();
     const int pieces = (a.N + 7) / 8;
     const int64_t count = (int64_t)a.T * pieces;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
@@ -1078,9 +1151,11 @@ __global__ void __launch_bounds__(256) k_gate_grad(const GradArgs a) {
         const int n = (int)(i - t * pieces) * 8;
         Eight<T> d, g, u;
         auto load = [&](Eight<T>& e, const void* p, int64_t ld) {
-            const T* row = reinterpret_cast<const T*>(p) + t * ld + n;
-            if (VEC && n + 8 <= a.N) e.load(row);
-            else e.load(row, a.N - n);
+            const T* all = reinterpret_cast<const T*>(p);
+            const T* row = all + t * ld + n;
+            if (n + 8 > a.N) e.load(row, a.N - n);
+            else if (VEC) e.load(row);
+            else e.load_any(row, all, all + (a.T - 1) * ld + a.N);
         };
         load(d, a.dh, a.ldd);
         load(g, a.g, a.ldg);
@@ -1108,9 +1183,22 @@ int bad(const char* msg) {
     return ABFT_ERR_ARG;
 }
 
-int launched(const char* what) {
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? ABFT_OK : cuda_fail(e, what);
+int status(cudaError_t e, const char* what) { return e == cudaSuccess ? ABFT_OK : cuda_fail(e, what); }
+
+// Launches a kernel that may start up while the one before it ends.
+template <typename... P, typename... A>
+cudaError_t launch_next(void (*kernel)(P...), dim3 grid, int block, int smem, cudaStream_t s, const A&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 // A row-major operand of elements of `size` bytes. One that bulk tensor copies
@@ -1123,20 +1211,6 @@ struct Operand {
     bool direct() const { return ((uintptr_t)p & 15) == 0 && (rows == 1 || (ld * size & 15) == 0); }
     int64_t packed_pitch() const { return cdiv((int64_t)cols * size, 16) * 16 / size; }
     size_t bytes() const { return direct() ? 0 : ((size_t)rows * packed_pitch() * size + 255) & ~(size_t)255; }
-
-    // In place of an operand that is not direct, its copy in `work`, which moves on.
-    void pack(char*& work, cudaStream_t s) {
-        if (direct()) return;
-        const dim3 grid((unsigned)std::min<int64_t>(rows, 4096), (unsigned)cdiv(cols, 256));
-        if (size == 1)
-            k_pack<<<grid, 256, 0, s>>>((const int8_t*)p, ld, rows, cols, (int8_t*)work, packed_pitch());
-        else
-            k_pack<<<grid, 256, 0, s>>>((const uint16_t*)p, ld, rows, cols, (uint16_t*)work, packed_pitch());
-        const size_t n = bytes();
-        p = work;
-        ld = packed_pitch();
-        work += n;
-    }
 
     // Boxes of 128 bytes x box_rows.
     bool map(CUtensorMap* m, int box_rows) const {
@@ -1152,6 +1226,33 @@ struct Operand {
     }
 };
 
+// Puts copies in `work` in place of the operands that are not direct; `work` moves on.
+cudaError_t pack(std::initializer_list<Operand*> operands, char*& work, cudaStream_t s) {
+    PackArgs a = {};
+    int n = 0, size = 0;
+    int64_t total = 0;
+    for (Operand* o : operands) {
+        if (o->direct()) continue;
+        a.in[n] = (const char*)o->p;
+        a.out[n] = work;
+        a.ld[n] = o->ld * o->size;
+        a.row[n] = (int64_t)o->cols * o->size;
+        a.rows[n] = o->rows;
+        a.chunks[n] = cdiv(a.row[n], 16);
+        total += a.rows[n] * a.chunks[n];
+        for (int i = n; i < 3; ++i) a.end[i] = total;
+        size = o->size;
+        const size_t bytes = o->bytes();
+        o->p = work;
+        o->ld = o->packed_pitch();
+        work += bytes;
+        ++n;
+    }
+    if (n == 0) return cudaSuccess;
+    const dim3 grid((unsigned)std::min<int64_t>(cdiv(total, 256), 148 * 32));
+    return size == 1 ? launch_next(k_pack<int8_t>, grid, 256, 0, s, a) : launch_next(k_pack<uint16_t>, grid, 256, 0, s, a);
+}
+
 // Number of SMs of the current device.
 int sm_count() {
     static std::atomic<int> cache[64];
@@ -1165,28 +1266,27 @@ int sm_count() {
 }
 
 // Threads per row and pieces held by each: the smallest that hold a row of K;
-// a warp alone needs no barrier. Unaligned rows are walked.
+// a warp alone needs no barrier.
 template <typename T>
-void quantize(const QuantArgs& a, cudaStream_t s) {
-    const bool vec = ((uintptr_t)a.x & 15) == 0 && (a.T == 1 || (a.ldx * (int64_t)sizeof(T) & 15) == 0) &&
-                     ((uintptr_t)a.q & 7) == 0 && (a.T == 1 || (a.ldq & 7) == 0) && ((uintptr_t)a.checksum & 15) == 0;
+cudaError_t quantize(QuantArgs a, cudaStream_t s) {
+    a.aligned = ((uintptr_t)a.x & 15) == 0 && (a.T == 1 || (a.ldx * (int64_t)sizeof(T) & 15) == 0) &&
+                ((uintptr_t)a.q & 7) == 0 && (a.T == 1 || (a.ldq & 7) == 0) && ((uintptr_t)a.checksum & 15) == 0;
     using std::integral_constant;
-    auto launch = [&](auto row, auto u, auto v, auto check) {
+    cudaError_t result = cudaSuccess;
+    auto launch = [&](auto row, auto u, auto check) {
         constexpr int kRow = decltype(row)::value, kU = decltype(u)::value, kBlock = kRow < 128 ? 128 : kRow;
-        // as many blocks as are resident at a time
         const int smem = decltype(check)::value && kU > 0 ? (int)cdiv(a.K, 8) * 32 : 0;
-        auto kernel = k_quantize_rows<T, kRow, kU, decltype(v)::value, decltype(check)::value>;
-        if (smem > 48 * 1024) (void)cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
+        auto kernel = k_quantize_rows<T, kRow, kU, decltype(check)::value>;
+        if (smem > 48 * 1024)
+            result = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
         int64_t blocks = cdiv(a.T, kBlock / kRow);
         if (blocks > sm_count()) {  // as many as are resident at a time, each with the same number of rows
             int resident = 1;
             if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kBlock, smem) != cudaSuccess) resident = 1;
             blocks = std::min<int64_t>(blocks, (int64_t)sm_count() * resident);
         }
-        kernel<<<(unsigned)blocks, kBlock, smem, s>>>(a);
+        if (result == cudaSuccess) result = launch_next(kernel, dim3((unsigned)blocks), kBlock, smem, s, a);
     };
-    const std::true_type yes;
-    const std::false_type no;
     const integral_constant<int, 32> warp;
     const integral_constant<int, 128> row128;
     const integral_constant<int, 256> row256;
@@ -1195,18 +1295,22 @@ void quantize(const QuantArgs& a, cudaStream_t s) {
     const integral_constant<int, 1> one;
     const integral_constant<int, 2> two;
     const integral_constant<int, 4> four;
+    const bool few = a.T <= sm_count();  // an SM for every row: more threads to a row
     auto choose = [&](auto check) {
-        if (!vec) a.K <= 1024 ? launch(warp, walk, no, check) : launch(row256, walk, no, check);
-        else if (a.K <= 256) launch(warp, one, yes, check);
-        else if (a.K <= 512) launch(warp, two, yes, check);
-        else if (a.K <= 1024) launch(warp, four, yes, check);
-        else if (a.K <= 2048) launch(row128, two, yes, check);
-        else if (a.K <= 4096) launch(row128, four, yes, check);
-        else if (a.K <= 8192) launch(row256, four, yes, check);
-        else if (a.K <= 16384) launch(row512, four, yes, check);
-        else launch(row512, walk, yes, check);
+        if (a.K <= 256) launch(warp, one, check);
+        else if (a.K <= 512) launch(warp, two, check);
+        else if (a.K <= 1024) launch(warp, four, check);
+        else if (few && a.K <= 4096) launch(row512, one, check);
+        else if (a.K <= 2048) launch(row128, two, check);
+        else if (a.K <= 4096) launch(row128, four, check);
+        else if (!few && a.K <= 8192) launch(row256, four, check);
+        else if (a.K <= 16384) launch(row512, four, check);
+        else launch(row512, walk, check);
     };
+    const std::true_type yes;
+    const std::false_type no;
     a.checksum ? choose(yes) : choose(no);
+    return result;
 }
 
 template <int MODE, int CG, int BN, bool SPLIT, typename O, int ACT>
@@ -1245,17 +1349,23 @@ int launch_product(const Operand (&a)[2], const Operand (&b)[2], ProductArgs arg
     cfg.blockDim = dim3(kProductThreads);
     cfg.dynamicSmemBytes = S::kSmem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = SPLIT ? args.split : CG;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = SPLIT ? args.split : CG;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     e = cudaLaunchKernelEx(&cfg, kernel, maps, args);
     return e == cudaSuccess ? ABFT_OK : cuda_fail(e, name);
 }
 
-constexpr int kFew = 32;  // tokens that k_few takes
+// Whether k_few takes a product of T tokens with `bytes` of weights: always up to
+// 16; up to 32 while the weights are small, since past that its own work shows
+// (block of 16384 x 4096, 32 tokens: 65 us, 48 tokens by k_product 49 us; block of
+// 1024 x 4096: 7.8 against 10.2 us).
+bool few_tokens(int T, int64_t bytes) { return T <= 16 || (T <= 32 && bytes <= 32 << 20); }
 
 template <bool GATE, typename E, typename O, int ACT = 0>
 int few(const Operand& x, const Operand (&w)[2], const ProductArgs& p, const char* name, cudaStream_t s) {
@@ -1274,14 +1384,30 @@ int few(const Operand& x, const Operand (&w)[2], const ProductArgs& p, const cha
     a.row_scale = p.row_scale;
     a.col_scale = p.col_scale;
     a.rowdiff = p.rowdiff;
-    const unsigned grid = (unsigned)cdiv(a.N, GATE ? 8 : 16);
-    if (a.T <= 8)
-        k_few<GATE, E, 1, O, ACT><<<grid, 256, 0, s>>>(a);
-    else if (a.T <= 16)
-        k_few<GATE, E, 2, O, ACT><<<grid, 256, 0, s>>>(a);
-    else
-        k_few<GATE, E, 4, O, ACT><<<grid, 256, 0, s>>>(a);
-    return launched(name);
+    // Warps that share a group's K: 8, so that a block streams whole rows, but none without a run of its own and 4 where
+    // more tokens make the warps' work longer than their wait (block of 16384 x 4096, one token: 46.9 / 43.3 / 44.9 / 39.9
+    // us with 1 / 2 / 4 / 8; 8-bit 8192 x 2048: 7.2 / 5.5 / 4.7 / 5.8; 16 tokens, block of 4096 x 4096: 28 / 17 / 14 / 16,
+    // of 1024 x 4096: 27 / 14 / 8.4 / 6.0).
+    const int64_t groups = cdiv(a.N, GATE ? 8 : 16);
+    const int most = a.T > 8 && groups >= sm_count() * 2 ? 4 : 8;
+    const int64_t run = a.T <= 16 ? 512 : 256;  // bytes of K that a warp takes at a time
+    int wk = 1;
+    while (wk < most && wk * run < a.kbytes) wk *= 2;
+    using std::integral_constant;
+    auto go = [&](auto nt, auto w) {
+        constexpr int kWk = decltype(w)::value;
+        return launch_next(k_few<GATE, E, decltype(nt)::value, kWk, O, ACT>, dim3((unsigned)cdiv(groups, 8 / kWk)), 256, 0,
+                           s, a);
+    };
+    auto with_wk = [&](auto nt) {
+        if (wk == 1) return go(nt, integral_constant<int, 1>());
+        if (wk == 2) return go(nt, integral_constant<int, 2>());
+        if (wk == 4) return go(nt, integral_constant<int, 4>());
+        return go(nt, integral_constant<int, 8>());
+    };
+    if (a.T <= 8) return status(with_wk(integral_constant<int, 1>()), name);
+    if (a.T <= 16) return status(with_wk(integral_constant<int, 2>()), name);
+    return status(with_wk(integral_constant<int, 4>()), name);
 }
 
 // Tile and split by an estimate in us: a start and an end that grow with the
@@ -1339,13 +1465,13 @@ int64_t grad_pitch(int N) { return (static_cast<int64_t>(N) + 7) / 8 * 8; }
 size_t grad_bytes(int T, int N) { return (static_cast<size_t>(T) * grad_pitch(N) * 2 + 255) & ~(size_t)255; }
 
 template <typename F>
-int with_type(int type, F&& f) {
+auto with_type(int type, F&& f) {
     if (type == ABFT_TYPE_F16) return f(__half());
     return f(__nv_bfloat16());
 }
 
 template <typename F>
-int with_act(int activation, F&& f) {
+auto with_act(int activation, F&& f) {
     if (activation == ABFT_ACT_SILU) return f(std::integral_constant<int, ABFT_ACT_SILU>());
     if (activation == ABFT_ACT_GELU) return f(std::integral_constant<int, ABFT_ACT_GELU>());
     return f(std::integral_constant<int, ABFT_ACT_GELU_TANH>());
@@ -1365,11 +1491,9 @@ int abft_quantize_rows(const void* dX, int64_t ldx, int type, int T, int K, int8
     if (T == 0) return ABFT_OK;
     if (!dX || !dQ || !dScale || (dChecksum != nullptr) != (dExpect != nullptr))
         return bad("abft_quantize_rows: bad argument (missing pointer, or one of dChecksum and dExpect alone)");
-    const QuantArgs args{dX, ldx, T, K, dQ, ldq, dScale, dChecksum, dExpect};
-    cudaStream_t s = (cudaStream_t)stream;
+    const QuantArgs args{false, dX, ldx, T, K, dQ, ldq, dScale, dChecksum, dExpect};
     auto go = [&](auto tag) {
-        quantize<decltype(tag)>(args, s);
-        return launched("abft_quantize_rows");
+        return status(quantize<decltype(tag)>(args, (cudaStream_t)stream), "abft_quantize_rows");
     };
     if (type == ABFT_TYPE_F32) return go(0.0f);
     return with_type(type, go);
@@ -1386,7 +1510,7 @@ int abft_column_checksum(const int8_t* dW, int64_t ldw, int N, int K, int32_t* d
         k_column_checksum<true><<<dim3((unsigned)cdiv(K, 1024), chunks), 256, 0, s>>>(dW, ldw, N, K, dChecksum);
     else
         k_column_checksum<false><<<dim3((unsigned)cdiv(K, 256), chunks), 256, 0, s>>>(dW, ldw, N, K, dChecksum);
-    return launched("abft_column_checksum");
+    return status(cudaGetLastError(), "abft_column_checksum");
 }
 
 size_t abft_int8_matmul_ws_bytes(const int8_t* dQ, int64_t ldq, const int8_t* dW, int64_t ldw, int T, int N, int K) {
@@ -1406,11 +1530,14 @@ int abft_int8_matmul(const int8_t* dQ, int64_t ldq, const float* dQScale, const 
         return bad("abft_int8_matmul: bad argument (missing pointer, or one of dExpect and dRowDiff alone)");
     if (work_bytes < abft_int8_matmul_ws_bytes(dQ, ldq, dW, ldw, T, N, K)) return bad("abft_int8_matmul: workspace too small");
     cudaStream_t s = (cudaStream_t)stream;
-    if (dExpect) k_negate<<<(unsigned)cdiv(T, 256), 256, 0, s>>>(dExpect, dRowDiff, T);
+    if (dExpect) {
+        const cudaError_t e = launch_next(k_negate, dim3((unsigned)cdiv(T, 256)), 256, 0, s, dExpect, dRowDiff, T);
+        if (e != cudaSuccess) return cuda_fail(e, "abft_int8_matmul");
+    }
     Operand q{dQ, ldq, T, K, 1}, w{dW, ldw, N, K, 1};
     char* work = (char*)dWork;
-    q.pack(work, s);
-    w.pack(work, s);
+    const cudaError_t packed = pack({&q, &w}, work, s);
+    if (packed != cudaSuccess) return cuda_fail(packed, "abft_int8_matmul");
     ProductArgs args = {};
     args.rows = T;
     args.cols = N;
@@ -1421,7 +1548,7 @@ int abft_int8_matmul(const int8_t* dQ, int64_t ldq, const float* dQScale, const 
     args.col_scale = dWScale;
     args.rowdiff = (unsigned long long*)dRowDiff;
     auto go = [&](auto tag) {
-        if (T <= kFew) return few<false, int8_t, decltype(tag)>(q, {w, w}, args, "abft_int8_matmul", s);
+        if (few_tokens(T, (int64_t)N * K)) return few<false, int8_t, decltype(tag)>(q, {w, w}, args, "abft_int8_matmul", s);
         return product<kInt8, decltype(tag)>({q, q}, {w, w}, args, "abft_int8_matmul", s);
     };
     if (type == ABFT_TYPE_F32) return go(0.0f);
@@ -1451,9 +1578,8 @@ int abft_gated_ffn(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg
     cudaStream_t s = (cudaStream_t)stream;
     Operand x{dX, ldx, T, K, 2}, wg{dWGate, ldwg, N, K, 2}, wu{dWUp, ldwu, N, K, 2};
     char* work = (char*)dWork;
-    x.pack(work, s);
-    wg.pack(work, s);
-    wu.pack(work, s);
+    const cudaError_t packed = pack({&x, &wg, &wu}, work, s);
+    if (packed != cudaSuccess) return cuda_fail(packed, "abft_gated_ffn");
     ProductArgs args = {};
     args.rows = T;
     args.cols = N;
@@ -1464,7 +1590,7 @@ int abft_gated_ffn(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg
     std::copy(pitches, pitches + 3, args.ld);
     return with_type(type, [&](auto tag) {
         return with_act(activation, [&](auto a) {
-            if (T <= kFew)
+            if (few_tokens(T, 4LL * N * K))
                 return few<true, decltype(tag), decltype(tag), decltype(a)::value>(x, {wg, wu}, args, "abft_gated_ffn", s);
             return product<kGate, decltype(tag), decltype(a)::value>({x, x}, {wg, wu}, args, "abft_gated_ffn", s);
         });
@@ -1503,22 +1629,19 @@ int abft_gated_ffn_backward(const void* dDH, int64_t ldd, const void* dX, int64_
     const Operand dg{work, p, T, N, 2}, du{work + grad_bytes(T, N), p, T, N, 2};
     work += 2 * grad_bytes(T, N);
     Operand x{dX, ldx, T, K, 2}, wg{dWGate, ldwg, N, K, 2}, wu{dWUp, ldwu, N, K, 2};
-    x.pack(work, s);
-    wg.pack(work, s);
-    wu.pack(work, s);
+    const cudaError_t packed = pack({&x, &wg, &wu}, work, s);
+    if (packed != cudaSuccess) return cuda_fail(packed, "abft_gated_ffn_backward");
     return with_type(type, [&](auto tag) {
         using E = decltype(tag);
-        with_act(activation, [&](auto a) {
+        const cudaError_t e = with_act(activation, [&](auto a) {
             const GradArgs ga{dDH, dG, dU, ldd, ldg, ldu, T, N, const_cast<void*>(dg.p), const_cast<void*>(du.p), p};
             const bool vec = Operand{dDH, ldd, T, N, 2}.direct() && Operand{dG, ldg, T, N, 2}.direct() &&
                              Operand{dU, ldu, T, N, 2}.direct();
             const unsigned grid = (unsigned)std::min<int64_t>(cdiv(T * cdiv(N, 8), 256), (int64_t)sm_count() * 64);
-            if (vec)
-                k_gate_grad<E, decltype(a)::value, true><<<grid, 256, 0, s>>>(ga);
-            else
-                k_gate_grad<E, decltype(a)::value, false><<<grid, 256, 0, s>>>(ga);
-            return 0;
+            return vec ? launch_next(k_gate_grad<E, decltype(a)::value, true>, dim3(grid), 256, 0, s, ga)
+                       : launch_next(k_gate_grad<E, decltype(a)::value, false>, dim3(grid), 256, 0, s, ga);
         });
+        if (e != cudaSuccess) return cuda_fail(e, "abft_gated_ffn_backward");
         ProductArgs args = {};
         args.rows = T;
         args.cols = K;
@@ -1532,8 +1655,7 @@ int abft_gated_ffn_backward(const void* dDH, int64_t ldd, const void* dX, int64_
         args.ld[0] = lddwg;
         args.c[1] = dDWUp;
         args.ld[1] = lddwu;
-        if (int rc = product<kDw, E>({dg, du}, {x, x}, args, "abft_gated_ffn_backward", s)) return rc;
-        return launched("abft_gated_ffn_backward");
+        return product<kDw, E>({dg, du}, {x, x}, args, "abft_gated_ffn_backward", s);
     });
 }
 

@@ -3,7 +3,8 @@
 Each function enqueues on a CUDA stream (default: the inputs' device's current
 stream) and returns immediately; matrices are row-major torch CUDA tensors
 (views with a row pitch are fine), weights are N x K. Outputs and scratch are
-allocated on that stream; inputs handed to a stream that is not the current
+allocated on that stream; the rows of an output whose width is not a multiple of
+8 (of q: 16) lie on a pitch that is; inputs handed to a stream that is not the current
 one are kept from reuse until its work is done. Nothing is kept between calls,
 so they can be captured into CUDA graphs and issued on several streams.
 """
@@ -92,7 +93,7 @@ def _empty8(rows, cols, device):
 
 
 def _empty16(rows, cols, dtype, device):
-    """A 16-bit matrix on a pitch of 16 bytes."""
+    """A matrix on a pitch of 8 elements (16 or 32 bytes)."""
     t = torch.empty((rows, (cols + 7) & ~7), dtype=dtype, device=device)
     return t[:, :cols] if cols & 7 else t
 
@@ -168,13 +169,13 @@ def int8_matmul(q, q_scale, w, w_scale, dtype=torch.bfloat16, expect=None, strea
         _vector(expect, "expect", torch.int64, T, dev)
     s, where = _on(dev, stream, (q, q_scale, w, w_scale, expect))
     with where:
-        y = torch.empty((T, N), dtype=dtype, device=dev)
+        y = _empty16(T, N, dtype, dev)
         rowdiff = None if expect is None else torch.empty(T, dtype=torch.int64, device=dev)
         qp, wp = q.data_ptr(), w.data_ptr()
         nbytes = lib.abft_int8_matmul_ws_bytes(qp, ldq, wp, ldw, T, N, K)
         work = _work(nbytes, dev)
-        rc = lib.abft_int8_matmul(qp, ldq, q_scale.data_ptr(), wp, ldw, w_scale.data_ptr(), T, N, K, y.data_ptr(), N,
-             TYPES[dtype], _ptr(expect), _ptr(rowdiff), _ptr(work), nbytes, s)
+        rc = lib.abft_int8_matmul(qp, ldq, q_scale.data_ptr(), wp, ldw, w_scale.data_ptr(), T, N, K, y.data_ptr(),
+             (N + 7) & ~7, TYPES[dtype], _ptr(expect), _ptr(rowdiff), _ptr(work), nbytes, s)
         if rc:
             check(rc, "abft_int8_matmul")
     return y if expect is None else (y, rowdiff)
@@ -235,15 +236,16 @@ def gated_ffn_backward(dh, x, w_gate, w_up, g, u, activation="silu", stream=None
     ldu = _matrix(u, "u", same, T, N, dev)
     s, where = _on(dev, stream, (dh, x, w_gate, w_up, g, u))
     with where:
-        dx = torch.empty((T, K), dtype=x.dtype, device=dev)
-        dw_gate = torch.empty((N, K), dtype=x.dtype, device=dev)
-        dw_up = torch.empty((N, K), dtype=x.dtype, device=dev)
+        dx = _empty16(T, K, x.dtype, dev)
+        dw_gate = _empty16(N, K, x.dtype, dev)
+        dw_up = _empty16(N, K, x.dtype, dev)
+        ld = (K + 7) & ~7
         xp, gp, up = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr()
         nbytes = lib.abft_gated_ffn_backward_ws_bytes(xp, ldx, gp, ldwg, up, ldwu, T, N, K)
         work = _work(nbytes, dev)
         rc = lib.abft_gated_ffn_backward(dh.data_ptr(), ldd, xp, ldx, gp, ldwg, up, ldwu, g.data_ptr(), ldg,
-             u.data_ptr(), ldu, T, N, K, TYPES[x.dtype], act, dx.data_ptr(), K, dw_gate.data_ptr(), K,
-             dw_up.data_ptr(), K, _ptr(work), nbytes, s)
+             u.data_ptr(), ldu, T, N, K, TYPES[x.dtype], act, dx.data_ptr(), ld, dw_gate.data_ptr(), ld,
+             dw_up.data_ptr(), ld, _ptr(work), nbytes, s)
         if rc:
             check(rc, "abft_gated_ffn_backward")
     return dx, dw_gate, dw_up
