@@ -23,28 +23,29 @@ INT8_MAX_ROWS = 1 << 24      # 127 * N fits a 32-bit checksum
 
 def _matrix(t, name, dtypes, rows=None, cols=None, device=None):
     """Checks a row-major CUDA matrix and returns its row pitch in elements."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.ndim == 2 and t.dtype in dtypes):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and t.ndim == 2):
         raise ValueError(f"{name} must be a 2-d CUDA tensor of {' or '.join(str(d)[6:] for d in dtypes)}")
     r, c = t.shape
     if (rows is not None and r != rows) or (cols is not None and c != cols):
-        raise ValueError(f"{name} is {tuple(t.shape)}, need ({'any' if rows is None else rows}, "
-                         f"{'any' if cols is None else cols})")
+        raise ValueError(f"{name} is {r} x {c}, need {'any' if rows is None else rows} x "
+                         f"{'any' if cols is None else cols}")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
     if c < 1 or r > 0x7fffffff or c > 0x7fffffff:
-        raise ValueError(f"{name} is {tuple(t.shape)}: rows of 1 to 2^31 - 1 elements are supported")
-    if c > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} is {r} x {c}: rows of 1 to 2^31 - 1 elements are supported")
+    pitch, step = t.stride()
+    if step != 1 and c > 1:
         raise ValueError(f"{name} must be row-major (stride 1 along a row)")
     if r <= 1:
         return (c + 15) & ~15  # one row has no pitch: any that keeps it aligned
-    if t.stride(0) < c:
-        raise ValueError(f"{name}'s rows overlap (row stride {t.stride(0)} < {c})")
-    return t.stride(0)
+    if pitch < c:
+        raise ValueError(f"{name}'s rows overlap (row stride {pitch} < {c})")
+    return pitch
 
 
 def _vector(t, name, dtype, n, device):
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype and t.shape == (n,)
-            and (n <= 1 or t.stride(0) == 1)):
+            and (t.is_contiguous() or n <= 1)):
         raise ValueError(f"{name} must be a contiguous CUDA vector of {n} {str(dtype)[6:]}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
@@ -86,16 +87,8 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _empty8(rows, cols, device):
-    """An 8-bit matrix on a pitch of 16 bytes."""
-    t = torch.empty((rows, (cols + 15) & ~15), dtype=torch.int8, device=device)
-    return t[:, :cols] if cols & 15 else t
-
-
-def _empty16(rows, cols, dtype, device):
-    """A matrix on a pitch of 8 elements (16 or 32 bytes)."""
-    t = torch.empty((rows, (cols + 7) & ~7), dtype=dtype, device=device)
-    return t[:, :cols] if cols & 7 else t
+def _empty(rows, cols, pitch, dtype, device):
+    return torch.empty_strided((rows, cols), (pitch, 1), dtype=dtype, device=device)
 
 
 def quantize_rows(x, checksum=None, stream=None):
@@ -118,7 +111,7 @@ def quantize_rows(x, checksum=None, stream=None):
         _vector(checksum, "checksum", torch.int32, K, dev)
     s, where = _on(dev, stream, (x, checksum))
     with where:
-        q = _empty8(T, K, dev)
+        q = _empty(T, K, (K + 15) & ~15, torch.int8, dev)
         scale = torch.empty(T, dtype=torch.float32, device=dev)
         expect = None if checksum is None else torch.empty(T, dtype=torch.int64, device=dev)
         rc = lib.abft_quantize_rows(x.data_ptr(), ldx, TYPES[x.dtype], T, K, q.data_ptr(), (K + 15) & ~15,
@@ -169,13 +162,15 @@ def int8_matmul(q, q_scale, w, w_scale, dtype=torch.bfloat16, expect=None, strea
         _vector(expect, "expect", torch.int64, T, dev)
     s, where = _on(dev, stream, (q, q_scale, w, w_scale, expect))
     with where:
-        y = _empty16(T, N, dtype, dev)
+        ld = (N + 7) & ~7
+        y = _empty(T, N, ld, dtype, dev)
         rowdiff = None if expect is None else torch.empty(T, dtype=torch.int64, device=dev)
         qp, wp = q.data_ptr(), w.data_ptr()
-        nbytes = lib.abft_int8_matmul_ws_bytes(qp, ldq, wp, ldw, T, N, K)
+        aligned = not ((qp | wp | ldq | ldw) & 15)  # then there is nothing to copy
+        nbytes = 0 if aligned else lib.abft_int8_matmul_ws_bytes(qp, ldq, wp, ldw, T, N, K)
         work = _work(nbytes, dev)
         rc = lib.abft_int8_matmul(qp, ldq, q_scale.data_ptr(), wp, ldw, w_scale.data_ptr(), T, N, K, y.data_ptr(),
-             (N + 7) & ~7, TYPES[dtype], _ptr(expect), _ptr(rowdiff), _ptr(work), nbytes, s)
+             ld, TYPES[dtype], _ptr(expect), _ptr(rowdiff), _ptr(work), nbytes, s)
         if rc:
             check(rc, "abft_int8_matmul")
     return y if expect is None else (y, rowdiff)
@@ -207,12 +202,13 @@ def gated_ffn(x, w_gate, w_up, activation="silu", save=False, stream=None):
     dev = x.device
     s, where = _on(dev, stream, (x, w_gate, w_up))
     with where:
-        h = _empty16(T, N, x.dtype, dev)
-        g = _empty16(T, N, x.dtype, dev) if save else None
-        u = _empty16(T, N, x.dtype, dev) if save else None
         ld = (N + 7) & ~7
+        h = _empty(T, N, ld, x.dtype, dev)
+        g = _empty(T, N, ld, x.dtype, dev) if save else None
+        u = _empty(T, N, ld, x.dtype, dev) if save else None
         xp, gp, up = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr()
-        nbytes = lib.abft_gated_ffn_ws_bytes(xp, ldx, gp, ldwg, up, ldwu, T, N, K)
+        aligned = not ((xp | gp | up) & 15 or (ldx | ldwg | ldwu) & 7)  # then there is nothing to copy
+        nbytes = 0 if aligned else lib.abft_gated_ffn_ws_bytes(xp, ldx, gp, ldwg, up, ldwu, T, N, K)
         work = _work(nbytes, dev)
         rc = lib.abft_gated_ffn(xp, ldx, gp, ldwg, up, ldwu, T, N, K, TYPES[x.dtype], act, h.data_ptr(), ld,
              _ptr(g), ld, _ptr(u), ld, _ptr(work), nbytes, s)
@@ -236,10 +232,10 @@ def gated_ffn_backward(dh, x, w_gate, w_up, g, u, activation="silu", stream=None
     ldu = _matrix(u, "u", same, T, N, dev)
     s, where = _on(dev, stream, (dh, x, w_gate, w_up, g, u))
     with where:
-        dx = _empty16(T, K, x.dtype, dev)
-        dw_gate = _empty16(N, K, x.dtype, dev)
-        dw_up = _empty16(N, K, x.dtype, dev)
         ld = (K + 7) & ~7
+        dx = _empty(T, K, ld, x.dtype, dev)
+        dw_gate = _empty(N, K, ld, x.dtype, dev)
+        dw_up = _empty(N, K, ld, x.dtype, dev)
         xp, gp, up = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr()
         nbytes = lib.abft_gated_ffn_backward_ws_bytes(xp, ldx, gp, ldwg, up, ldwu, T, N, K)
         work = _work(nbytes, dev)
