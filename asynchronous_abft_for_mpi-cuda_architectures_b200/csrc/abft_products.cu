@@ -495,8 +495,7 @@ struct ProductArgs {
     bool wide[3];                // 16-byte stores are possible
     const float* row_scale;
     const float* col_scale;
-    unsigned long long* rowdiff;  // zeroed before; the tile of a row's first columns subtracts what is expected
-    const int64_t* expect;
+    unsigned long long* rowdiff;  // holds minus what is expected
 };
 
 struct ProductMaps {
@@ -788,7 +787,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
                 tensor::tc_fence_before();
                 __syncwarp();
                 if (lane == 0)
-                    tensor::bar_arrive_cluster(CG == 2 ? tensor::in_leader(sums_empty(buf)) : sums_empty(buf));
+                    tensor::bar_arrive(CG == 2 ? tensor::in_leader(sums_empty(buf)) : sums_empty(buf));
             };
             if (!SPLIT && j0 == j1) taken();
 #pragma unroll 1
@@ -834,10 +833,8 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
                 }
             }
             // sums of columns and rows beyond the matrices are zeros
-            if (MODE == kInt8 && !SPLIT && lane < rows && a.rowdiff) {
-                if (n0 == 0 && half == 0) total -= a.expect[m0 + lane];
+            if (MODE == kInt8 && !SPLIT && lane < rows && a.rowdiff)
                 atomicAdd(a.rowdiff + m0 + lane, static_cast<unsigned long long>(total));
-            }
         }
     }
     __syncwarp();
@@ -857,7 +854,8 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
             out = 1;
         }
         constexpr int kFours = S::kCols / 4;  // threads of a row, 32 at most
-        const int n0 = nt * S::kCols, share = 128 / a.split;
+        const int n0 = nt * S::kCols;
+        const int r0 = 128 * (int)in_cluster / a.split, r1 = 128 * ((int)in_cluster + 1) / a.split;
         auto sum = [&](int r, int c, auto(&v)[4]) {
             uint4 part[8];
 #pragma unroll
@@ -888,11 +886,11 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
                     if (n0 + c + j < a.cols) to[j] = from_f32<O>(v[j]);
             }
         };
-        // whole warps go round together: share * kFours is a multiple of 32
-        for (int e = threadIdx.x; e < share * kFours; e += kProductThreads) {
-            const int r = (int)in_cluster * share + e / kFours, c = e % kFours * 4;
+        // whole warps go round together, the last with rows of the next share that it leaves alone
+        for (int e = threadIdx.x; e < ((r1 - r0) * kFours + 31) / 32 * 32; e += kProductThreads) {
+            const int r = min(r0 + e / kFours, 127), c = e % kFours * 4;
             const int64_t m = mt * 128 + r;
-            const bool live = m < a.rows;
+            const bool live = r0 + e / kFours < r1 && m < a.rows;
             if constexpr (MODE == kInt8) {
                 int v[4] = {};
                 sum(r, c, v);
@@ -906,10 +904,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
                     long long total = (long long)v[0] + v[1] + v[2] + v[3];
 #pragma unroll
                     for (int o = kFours / 2; o; o >>= 1) total += __shfl_down_sync(~0u, total, o, kFours);
-                    if (c == 0 && live) {
-                        if (n0 == 0) total -= a.expect[m];
-                        atomicAdd(a.rowdiff + m, static_cast<unsigned long long>(total));
-                    }
+                    if (c == 0 && live) atomicAdd(a.rowdiff + m, static_cast<unsigned long long>(total));
                 }
             } else if constexpr (MODE == kGate) {
                 float g[4] = {}, up[4] = {};
@@ -979,7 +974,6 @@ struct FewArgs {
     const float* row_scale;
     const float* col_scale;
     unsigned long long* rowdiff;
-    const int64_t* expect;
 };
 
 // 16 bytes at byte `off` of a row of `n` bytes, zeros beyond it; weights pass L1 by.
@@ -1079,10 +1073,7 @@ __global__ void __launch_bounds__(256, 2) k_few(const FewArgs a) {
             if (a.rowdiff) {
                 long long sum = (in0 ? (long long)s0 : 0) + (in1 ? (long long)s1 : 0);
                 for (int o = 4; o; o >>= 1) sum += __shfl_down_sync(~0u, sum, o, 8);
-                if (ch == 0 && tok < a.T) {
-                    if (n == 0) sum -= a.expect[tok];
-                    atomicAdd(a.rowdiff + tok, static_cast<unsigned long long>(sum));
-                }
+                if (ch == 0 && tok < a.T) atomicAdd(a.rowdiff + tok, static_cast<unsigned long long>(sum));
             }
         } else {
             float gate = 0.0f, up = 0.0f;
@@ -1100,6 +1091,17 @@ __global__ void __launch_bounds__(256, 2) k_few(const FewArgs a) {
             }
         }
     }
+}
+
+// What the rows' sums are added to. A kernel that starts beside the one before it
+// rather than a memset, which would end that: one quantised and verified token,
+// 16384 x 4096, replayed from a graph: 12.9 us against 16.1 (called eagerly, where
+// the host's 27 us are the bound, the memset saves 1.5 us).
+__global__ void __launch_bounds__(256) k_negate(const int64_t* __restrict__ in, int64_t* __restrict__ out, int n) {
+    tensor::wait_for_stream();
+    tensor::let_next_start();
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) out[i] = -in[i];
 }
 
 // Rows of up to three matrices onto another pitch, 16 bytes a thread.
@@ -1391,7 +1393,6 @@ int few(const Operand& x, const Operand (&w)[2], const ProductArgs& p, const cha
     a.row_scale = p.row_scale;
     a.col_scale = p.col_scale;
     a.rowdiff = p.rowdiff;
-    a.expect = p.expect;
     // Warps that share a group's K: 8, so that a block streams whole rows, but none without a run of its own and 4 where
     // more tokens make the warps' work longer than their wait (block of 16384 x 4096, one token: 46.9 / 43.3 / 44.9 / 39.9
     // us with 1 / 2 / 4 / 8; 8-bit 8192 x 2048: 7.2 / 5.5 / 4.7 / 5.8; 16 tokens, block of 4096 x 4096: 28 / 17 / 14 / 16,
@@ -1418,22 +1419,50 @@ int few(const Operand& x, const Operand (&w)[2], const ProductArgs& p, const cha
     return status(with_wk(integral_constant<int, 4>()), name);
 }
 
-// Tile and split by an estimate in us: a start and an end that grow with the
-// tile, and for every round of tiles its chunks of 128 bytes of K, a chunk
-// costing what it does on a busy GPU:
+// Clusters of `split` product CTAs (one an SM) that the GPU runs at a time; SMs
+// come in groups that a cluster does not leave, so this is below SMs / split.
+int clusters_at_once(int split) {
+    static std::atomic<int> cache[64][9];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev > 63) return 0;
+    int n = cache[dev][split].load();
+    if (n) return n - 1;
+    using S = Shape<kInt8, 1, 128, float>;
+    auto kernel = k_product<kInt8, 1, 128, true, float, 0>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(split);
+    cfg.blockDim = dim3(kProductThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return 0;
+    }
+    cache[dev][split].store(n + 1);
+    return n;
+}
+
+// Tile and split by an estimate in us: a start and an end, and for every round of
+// tiles its chunks of 128 bytes of K or its results on their way out, whichever
+// is longer:
 //
-//                       start + end   a chunk   (measured alone / all SMs busy)
-//   pair of SMs, 256        7.0        0.31      0.28 / 0.34
-//   one SM, 128 columns     5.0        0.21      0.18 / 0.24
-//   one SM, 64 columns      4.4        0.19      0.17 / 0.22
-//   split, 128 columns      7.2        0.20      for all CTAs at once only
-//   split, 64 columns       6.7        0.19
+//                       start + end   a chunk (alone / all SMs busy)   32 x 32 results of a warp
+//   pair of SMs, 256        5.2        0.30  (0.28 / 0.31)              4 x 0.45
+//   one SM, 128 columns     4.0        0.20  (0.19 / 0.21)              2 x 0.45
+//   one SM, 64 columns      4.0        0.185 (0.18 / 0.19)              1 x 0.45
+//   split, 128 columns      7.2        0.20   all clusters at once only
+//   split, 64 columns       6.8        0.18
 //
-// Examples, bf16 block, us measured (256 / 128 / 64 / best split): 8192 x 16384 x
-// 4096 1540 / 2288 / - / -; 512 x 4096 x 4096 27 / 34 / 53 / 56; 2048 x 1536 x 1024
-// 16.7 / 15.7 / 23.9 / 49; 128 x 1536 x 1024 11.0 / 7.7 / 7.3 / 8.3; 128 x 4096 x 4096
-// 24.9 / 17.5 / 16.6 / 14.3; 128 x 1024 x 4096 24.3 / 16.7 / 15.9 / 10.3. Clusters of 8
-// do not fill the GPU (13 us where 4 take 8), so they stay at 64 CTAs.
+// Examples, us measured (pair / 128 / 64 / best split): bf16 block of 8192 tokens,
+// 16384 x 4096: 1540 / 2288 / - / -; 1000, 4096 x 4096: 45 / 58 / 88 / -; 1000, 1536 x
+// 1024: 10.8 / 11.1 / 14.1 / -; 48, 1536 x 1024: 9.2 / 6.8 / 7.0 / 7.6; 48, 4096 x 4096:
+// 23.2 / 16.6 / 16.3 / 13.3; 48, 512 x 16384: 76 / 52 / 50 / 14.
 template <int MODE, typename O, int ACT = 0>
 int product(const Operand (&a)[2], const Operand (&b)[2], ProductArgs args, const char* name, cudaStream_t s) {
     const int chunks = args.chunks * (MODE == kDx ? 2 : 1);
@@ -1441,23 +1470,25 @@ int product(const Operand (&a)[2], const Operand (&b)[2], ProductArgs args, cons
         return (MODE == kDw ? 2 : 1) * cdiv(args.rows, rows) * cdiv(args.cols, MODE == kGate ? columns / 2 : columns);
     };
     const int sms = sm_count();
+    const int outputs = args.c[1] && MODE == kGate ? 3 : MODE == kGate ? 1 : 2;  // in halves of a tile
     double best = 1e30;
     int which = 0;
-    auto consider = [&](int i, int split, double ends, double chunk, int64_t rounds) {
-        const double us = ends + chunk * (double)rounds * (double)cdiv(chunks, split);
+    auto consider = [&](int i, int split, double ends, double chunk, int columns, int64_t rounds) {
+        const double round = std::max(chunk * (double)cdiv(chunks, split), 0.45 / 128 * columns * outputs);
+        const double us = ends + round * (double)rounds;
         if (us < best) {
             best = us;
             which = i;
             args.split = split;
         }
     };
-    consider(0, 1, 7.0, 0.31, cdiv(tiles(256, 256), std::max(sms / 2, 1)));
-    consider(1, 1, 5.0, 0.21, cdiv(tiles(128, 128), sms));
-    consider(2, 1, 4.4, 0.19, cdiv(tiles(128, 64), sms));
-    for (int split = 2; split <= 8 && split <= chunks; split *= 2) {
-        const int most = split == 8 ? 64 : std::min(sms, 128);
-        if (tiles(128, 128) * split <= most) consider(3, split, 7.2, 0.20, 1);
-        if (tiles(128, 64) * split <= most) consider(4, split, 6.7, 0.19, 1);
+    consider(0, 1, 5.2, 0.30, 256, cdiv(tiles(256, 256), std::max(sms / 2, 1)));
+    consider(1, 1, 4.0, 0.20, 128, cdiv(tiles(128, 128), sms));
+    consider(2, 1, 4.0, 0.185, 64, cdiv(tiles(128, 64), sms));
+    for (int split = 2; split <= 8 && split <= chunks && tiles(128, 128) * split <= sms; ++split) {
+        const int clusters = clusters_at_once(split);
+        if (tiles(128, 128) <= clusters) consider(3, split, 7.2, 0.20, 0, 1);
+        if (tiles(128, 64) <= clusters) consider(4, split, 6.8, 0.18, 0, 1);
     }
     switch (which) {
         case 0: return launch_product<MODE, 2, 256, false, O, ACT>(a, b, args, name, s);
@@ -1539,7 +1570,7 @@ int abft_int8_matmul(const int8_t* dQ, int64_t ldq, const float* dQScale, const 
     if (work_bytes < abft_int8_matmul_ws_bytes(dQ, ldq, dW, ldw, T, N, K)) return bad("abft_int8_matmul: workspace too small");
     cudaStream_t s = (cudaStream_t)stream;
     if (dExpect) {
-        const cudaError_t e = cudaMemsetAsync(dRowDiff, 0, sizeof(int64_t) * T, s);
+        const cudaError_t e = launch_next(k_negate, dim3((unsigned)cdiv(T, 256)), 256, 0, s, dExpect, dRowDiff, T);
         if (e != cudaSuccess) return cuda_fail(e, "abft_int8_matmul");
     }
     Operand q{dQ, ldq, T, K, 1}, w{dW, ldw, N, K, 1};
@@ -1555,7 +1586,6 @@ int abft_int8_matmul(const int8_t* dQ, int64_t ldq, const float* dQScale, const 
     args.row_scale = dQScale;
     args.col_scale = dWScale;
     args.rowdiff = (unsigned long long*)dRowDiff;
-    args.expect = dExpect;
     auto go = [&](auto tag) {
         if (few_tokens(T, (int64_t)N * K)) return few<false, int8_t, decltype(tag)>(q, {w, w}, args, "abft_int8_matmul", s);
         return product<kInt8, decltype(tag)>({q, q}, {w, w}, args, "abft_int8_matmul", s);
