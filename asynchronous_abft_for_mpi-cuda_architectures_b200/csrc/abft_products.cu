@@ -568,14 +568,29 @@ __device__ __forceinline__ void store_block(char* mine, O* to, int64_t ld, int r
     __syncwarp();
     if (wide && cols >= 32) {
         const int r = lane / kPieces, piece = lane % kPieces;
+        uint4 out[kPieces];
 #pragma unroll
-        for (int i = 0; i < 32; i += 32 / kPieces)
-            if (i + r < rows)
-                *reinterpret_cast<uint4*>(to + (i + r) * ld + piece * kV) =
-                    *reinterpret_cast<uint4*>(mine + (i + r) * kPitch + piece * 16);
+        for (int i = 0; i < kPieces; ++i)
+            out[i] = *reinterpret_cast<const uint4*>(mine + (i * (32 / kPieces) + r) * kPitch + piece * 16);
+        to += r * ld + piece * kV;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+            if (i * (32 / kPieces) + r < rows) *reinterpret_cast<uint4*>(to + i * (32 / kPieces) * ld) = out[i];
     } else if (lane < cols) {
-        for (int i = 0; i < 32 && i < rows; ++i)
-            to[i * ld + lane] = *reinterpret_cast<O*>(mine + i * kPitch + lane * sizeof(O));
+        to += lane;
+        const char* from = mine + lane * sizeof(O);
+#pragma unroll 1
+        for (int i = 0; i < 32 && i < rows; i += 4) {
+            O out[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[j] = *reinterpret_cast<const O*>(from + j * kPitch);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (i + j < rows) *to = out[j];
+                to += ld;
+            }
+            from += 4 * kPitch;
+        }
     }
 }
 
@@ -585,7 +600,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
     constexpr int kPart = BN + 4;  // SPLIT: pitch of the partial sums, which overlay the stages
     static_assert(!SPLIT || CG == 1, "a split tile is one CTA wide");
     extern __shared__ char raw[];
-    char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    char* smem = raw + (-tensor::smem_u32(raw) & 1023);
     const uint32_t base = tensor::smem_u32(smem);
     const uint32_t bars = base + S::kBars;
     auto full = [&](int s) { return bars + 8 * s; };
@@ -780,8 +795,10 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
             if (!__all_sync(~0u, wait_for(sums_full(buf), (n >> 1) & 1, a.limit, stop))) break;
             tensor::tc_fence_after();
             auto put = [&](int i, int j, const float(&v)[32]) {
-                store_block<O>(mine, reinterpret_cast<O*>(a.c[i]) + m0 * a.ld[i] + n0 + j, a.ld[i], rows,
-                               a.cols - n0 - j, a.wide[i], v);
+                const int64_t ld = i == 0 ? a.ld[0] : i == 1 ? a.ld[1] : a.ld[2];
+                void* c = i == 0 ? a.c[0] : i == 1 ? a.c[1] : a.c[2];
+                const bool wide = i == 0 ? a.wide[0] : i == 1 ? a.wide[1] : a.wide[2];
+                store_block<O>(mine, reinterpret_cast<O*>(c) + m0 * ld + n0 + j, ld, rows, a.cols - n0 - j, wide, v);
             };
             auto taken = [&] {  // the sums are out: the next tile may overwrite them
                 tensor::tc_fence_before();
@@ -806,10 +823,15 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
                     for (int i = 0; i < 8; ++i) part[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
                 } else if constexpr (MODE == kInt8) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int sum = static_cast<int>(r[i]);
-                        total += sum;
-                        v[i] = static_cast<float>(sum) * rs * sc[j - j0 + i];
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 cs = *reinterpret_cast<const float4*>(sc + j - j0 + i);
+                        const float scale[4] = {cs.x, cs.y, cs.z, cs.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int sum = static_cast<int>(r[i + k]);
+                            total += sum;
+                            v[i + k] = static_cast<float>(sum) * rs * scale[k];
+                        }
                     }
                     put(0, j, v);
                 } else if constexpr (MODE == kGate) {
@@ -840,7 +862,8 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
     __syncwarp();
     tensor::tc_fence_before();
     __syncthreads();
-    if constexpr (CG == 2 || SPLIT) tensor::cluster_sync();
+    if constexpr (SPLIT) tensor::cluster_sync();           // the partial sums are there
+    if constexpr (CG == 2) tensor::cluster_sync_relaxed();  // the leader's instructions use both CTAs' memory
     tensor::tc_fence_after();
     if (warp == 2) tensor::tmem_free<CG>(tmem, S::kTmemCols);
 
@@ -873,8 +896,11 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
                 }
         };
         auto put = [&](int i, int64_t m, int c, const float(&v)[4]) {
-            O* to = reinterpret_cast<O*>(a.c[i]) + m * a.ld[i] + n0 + c;
-            if (a.wide[i] && n0 + c + 4 <= a.cols) {
+            const int64_t ld = i == 0 ? a.ld[0] : i == 1 ? a.ld[1] : a.ld[2];
+            void* all = i == 0 ? a.c[0] : i == 1 ? a.c[1] : a.c[2];
+            const bool wide = i == 0 ? a.wide[0] : i == 1 ? a.wide[1] : a.wide[2];
+            O* to = reinterpret_cast<O*>(all) + m * ld + n0 + c;
+            if (wide && n0 + c + 4 <= a.cols) {
                 alignas(16) O pack[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) pack[j] = from_f32<O>(v[j]);
@@ -926,7 +952,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
             }
         }
         __syncwarp();
-        tensor::cluster_sync();  // the others still read this CTA's sums
+        tensor::cluster_sync_relaxed();  // the others still read this CTA's sums
     }
 }
 

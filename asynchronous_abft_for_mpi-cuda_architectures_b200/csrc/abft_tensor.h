@@ -48,6 +48,12 @@ __device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
     return r;
 }
 
+// All threads of the cluster, without waiting for their stores to global memory:
+// for what only has to outlive the others' reads and instructions.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+}
+
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
