@@ -473,8 +473,9 @@ __global__ void __launch_bounds__(256) k_column_checksum(const int8_t* __restric
 // writes whole 64- or 128-byte runs of each output row, aligned or not.
 //
 // SPLIT: when there are too few tiles for the GPU, the CTAs of a cluster share
-// one tile's K; their partial sums meet in shared memory (each CTA adds up its
-// share of the rows in a fixed order, reading the others' over the cluster).
+// one tile's K. Each sends its partial sums of a row to the CTA that writes that
+// row (stores over the cluster; reading them there instead took 2 us more), which
+// adds them up in a fixed order.
 //
 // Nothing is transposed in memory: an operand whose summed index runs along
 // the pitch is MN-major, which the matrix instructions read directly. Rows and
@@ -507,7 +508,7 @@ __device__ unsigned g_fault;
 
 constexpr int kProductThreads = 384;  // copies, matrix instructions, 2 idle warps (one holds tensor memory), 8 for results
 
-template <int MODE, int CG, int BN, typename O>
+template <int MODE, int CG, int BN, bool SPLIT, typename O>
 struct Shape {
     static constexpr bool kTwoPairs = MODE == kDx;
     static constexpr bool kAMn = MODE == kDw;
@@ -517,14 +518,20 @@ struct Shape {
     static constexpr int kStageBytes = kABytes + kBBytes;
     static constexpr int kOutBytes = 32 * (32 * (int)sizeof(O) + 16);  // 32 x 32 results on their way out, one warp
     // 227 KB of shared memory: alignment, barriers, 8 warps' results and channel scales; the rest are stages
-    static constexpr int kRoom = 227 * 1024 - 1024 - 512 - 8 * kOutBytes - 8 * 128 * 4;
+    static constexpr int kOutRoom = SPLIT ? 0 : 8 * kOutBytes;
+    static constexpr int kRoom = 227 * 1024 - 1024 - 512 - kOutRoom - 8 * 128 * 4;
+    // SPLIT: pitch of partial sums, which overlay the stages (128 rows and at most 8 more, see share_rows)
+    static constexpr int kPart = BN + 4;
     static constexpr int kStages = kRoom / kStageBytes < 8 ? kRoom / kStageBytes : 8;
     static constexpr int kOut = kStages * kStageBytes;
-    static constexpr int kScales = kOut + 8 * kOutBytes;
+    static constexpr int kScales = kOut + kOutRoom;
     static constexpr int kBars = kScales + 8 * 128 * 4;
     static constexpr int kSmem = 1024 + kBars + 512;
     static constexpr int kTmemCols = 2 * BN;
 };
+
+// SPLIT: rows of the largest share of a tile, at most.
+__device__ __forceinline__ int share_rows(int split) { return 128 / split + (128 % split != 0); }
 
 // A wait with a limit. `stop` is set for the whole CTA by the first that runs out.
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, int limit, volatile int* stop) {
@@ -596,8 +603,8 @@ __device__ __forceinline__ void store_block(char* mine, O* to, int64_t ld, int r
 
 template <int MODE, int CG, int BN, bool SPLIT, typename O, int ACT>
 __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_constant__ ProductMaps maps, const ProductArgs a) {
-    using S = Shape<MODE, CG, BN, O>;
-    constexpr int kPart = BN + 4;  // SPLIT: pitch of the partial sums, which overlay the stages
+    using S = Shape<MODE, CG, BN, SPLIT, O>;
+    static_assert(!SPLIT || (128 + 8) * S::kPart * 4 <= S::kOut, "the partial sums fit the stages");
     static_assert(!SPLIT || CG == 1, "a split tile is one CTA wide");
     extern __shared__ char raw[];
     char* smem = raw + (-tensor::smem_u32(raw) & 1023);
@@ -638,8 +645,9 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
     }
     if (warp == 2) tensor::tmem_alloc<CG>(tensor::smem_u32(const_cast<uint32_t*>(tmem_slot)), S::kTmemCols);
     tensor::tc_fence_before();
-    __syncthreads();
     if constexpr (CG == 2) tensor::cluster_sync();
+    else __syncthreads();
+    if (SPLIT && warp < 4) tensor::cluster_arrive_relaxed();
     tensor::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     tensor::wait_for_stream();
@@ -770,6 +778,12 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
         const int j0 = half ? (kBlocks + 1) / 2 * 32 : 0, j1 = half ? kBlocks * 32 : (kBlocks + 1) / 2 * 32;
         const uint32_t lanes = tmem + ((uint32_t)w << 21);
         char* mine = smem + S::kOut + (warp - 4) * S::kOutBytes;
+        // SPLIT: this lane's row belongs to CTA `owner`, from whose first row on it is row `in_share`
+        const int owner = SPLIT ? ((w * 32 + lane + 1) * a.split - 1) / 128 : 0;
+        const int in_share = w * 32 + lane - (SPLIT ? 128 * owner / a.split : 0);
+        uint32_t part = 0;
+        if constexpr (SPLIT)
+            part = tensor::in_cta(base + ((int)in_cluster * share_rows(a.split) + in_share) * S::kPart * 4, owner);
         float* sc = reinterpret_cast<float*>(smem + S::kScales) + (warp - 4) * 128;
         int n = 0;
         for (int tile = first; tile < tiles; tile += step, ++n) {
@@ -792,7 +806,12 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
                 for (int j = j0 + lane; j < j1; j += 32) sc[j - j0] = n0 + j < a.cols ? a.col_scale[n0 + j] : 0.0f;
                 __syncwarp();
             }
-            if (!__all_sync(~0u, wait_for(sums_full(buf), (n >> 1) & 1, a.limit, stop))) break;
+            const bool ok = __all_sync(~0u, wait_for(sums_full(buf), (n >> 1) & 1, a.limit, stop));
+            if constexpr (SPLIT) {  // no CTA's instructions read their stages any more
+                tensor::cluster_arrive_relaxed();
+                tensor::cluster_wait();
+            }
+            if (!ok) break;
             tensor::tc_fence_after();
             auto put = [&](int i, int j, const float(&v)[32]) {
                 const int64_t ld = i == 0 ? a.ld[0] : i == 1 ? a.ld[1] : a.ld[2];
@@ -818,9 +837,8 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
                 if (!SPLIT && j + 32 == j1) taken();
                 float v[32];
                 if constexpr (SPLIT) {
-                    uint4* part = reinterpret_cast<uint4*>(smem + ((w * 32 + lane) * kPart + j) * 4);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) part[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+                    for (int i = 0; i < 32; i += 4) tensor::store_cluster(part + (j + i) * 4, r[i], r[i + 1], r[i + 2], r[i + 3]);
                 } else if constexpr (MODE == kInt8) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
@@ -861,14 +879,20 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
     }
     __syncwarp();
     tensor::tc_fence_before();
-    __syncthreads();
-    if constexpr (SPLIT) tensor::cluster_sync();           // the partial sums are there
-    if constexpr (CG == 2) tensor::cluster_sync_relaxed();  // the leader's instructions use both CTAs' memory
+    if constexpr (SPLIT) {
+        if (warp < 4) tensor::cluster_wait();
+        tensor::cluster_sync();  // the partial sums are there
+    } else if constexpr (CG == 2) {  // the leader's instructions use both CTAs' memory; nothing waits for their stores
+        tensor::cluster_arrive_relaxed();
+        tensor::cluster_wait();
+    } else {
+        __syncthreads();
+    }
     tensor::tc_fence_after();
     if (warp == 2) tensor::tmem_free<CG>(tmem, S::kTmemCols);
 
     if constexpr (SPLIT) {
-        // every CTA adds up its share of the tile's rows: a thread takes 4 columns of a row, all CTAs' parts of them at once
+        // every CTA adds up its share of the tile's rows: a thread takes 4 columns of a row
         int mt, nt;
         tile_at(first, a.tiles_m, a.tiles_n, mt, nt);
         int out = 0;
@@ -879,21 +903,19 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
         constexpr int kFours = S::kCols / 4;  // threads of a row, 32 at most
         const int n0 = nt * S::kCols;
         const int r0 = 128 * (int)in_cluster / a.split, r1 = 128 * ((int)in_cluster + 1) / a.split;
+        const int rows = share_rows(a.split);
         auto sum = [&](int r, int c, auto(&v)[4]) {
-            uint4 part[8];
-#pragma unroll
-            for (int p = 0; p < 8; ++p)
-                if (p < a.split) part[p] = tensor::load_from(base + (r * kPart + c) * 4, p);
-#pragma unroll
-            for (int p = 0; p < 8; ++p)
-                if (p < a.split) {
-                    const uint32_t q[4] = {part[p].x, part[p].y, part[p].z, part[p].w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (MODE == kInt8) v[i] += static_cast<int>(q[i]);
-                        else v[i] += __uint_as_float(q[i]);
-                    }
+            const char* at = smem + ((r - r0) * S::kPart + c) * 4;
+#pragma unroll 4
+            for (int p = 0; p < a.split; ++p) {
+                const uint4 q = *reinterpret_cast<const uint4*>(at + p * rows * S::kPart * 4);
+                if constexpr (MODE == kInt8) {
+                    v[0] += (int)q.x, v[1] += (int)q.y, v[2] += (int)q.z, v[3] += (int)q.w;
+                } else {
+                    v[0] += __uint_as_float(q.x), v[1] += __uint_as_float(q.y);
+                    v[2] += __uint_as_float(q.z), v[3] += __uint_as_float(q.w);
                 }
+            }
         };
         auto put = [&](int i, int64_t m, int c, const float(&v)[4]) {
             const int64_t ld = i == 0 ? a.ld[0] : i == 1 ? a.ld[1] : a.ld[2];
@@ -914,7 +936,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
         };
         // whole warps go round together, the last with rows of the next share that it leaves alone
         for (int e = threadIdx.x; e < ((r1 - r0) * kFours + 31) / 32 * 32; e += kProductThreads) {
-            const int r = min(r0 + e / kFours, 127), c = e % kFours * 4;
+            const int r = min(r0 + e / kFours, r1 - 1), c = e % kFours * 4;
             const int64_t m = mt * 128 + r;
             const bool live = r0 + e / kFours < r1 && m < a.rows;
             if constexpr (MODE == kInt8) {
@@ -951,8 +973,6 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
                 if (live) put(out, m, c, v);
             }
         }
-        __syncwarp();
-        tensor::cluster_sync_relaxed();  // the others still read this CTA's sums
     }
 }
 
@@ -1350,7 +1370,7 @@ cudaError_t quantize(QuantArgs a, cudaStream_t s) {
 
 template <int MODE, int CG, int BN, bool SPLIT, typename O, int ACT>
 int launch_product(const Operand (&a)[2], const Operand (&b)[2], ProductArgs args, const char* name, cudaStream_t s) {
-    using S = Shape<MODE, CG, BN, O>;
+    using S = Shape<MODE, CG, BN, SPLIT, O>;
     ProductMaps maps;
     const int b_box = S::kBMn ? 64 : MODE == kGate ? BN / 2 : BN / CG;
     const int a_box = S::kAMn ? 64 : 128;
@@ -1453,7 +1473,7 @@ int clusters_at_once(int split) {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev > 63) return 0;
     int n = cache[dev][split].load();
     if (n) return n - 1;
-    using S = Shape<kInt8, 1, 128, float>;
+    using S = Shape<kInt8, 1, 128, true, float>;
     auto kernel = k_product<kInt8, 1, 128, true, float, 0>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(split);
@@ -1481,9 +1501,9 @@ int clusters_at_once(int split) {
 //                       start + end   a chunk (alone / all SMs busy)   32 x 32 results of a warp
 //   pair of SMs, 256        5.2        0.30  (0.28 / 0.31)              4 x 0.45
 //   one SM, 128 columns     4.0        0.20  (0.19 / 0.21)              2 x 0.45
-//   one SM, 64 columns      4.0        0.185 (0.18 / 0.19)              1 x 0.45
-//   split, 128 columns      7.2        0.20   all clusters at once only
-//   split, 64 columns       6.8        0.18
+//   one SM, 64 columns      4.0        0.185 (0.18 / 0.19)             1 x 0.45
+//   split, 128 columns      7.3        0.20   all clusters at once only
+//   split, 64 columns       5.8        0.18
 //
 // Examples, us measured (pair / 128 / 64 / best split): bf16 block of 8192 tokens,
 // 16384 x 4096: 1540 / 2288 / - / -; 1000, 4096 x 4096: 45 / 58 / 88 / -; 1000, 1536 x
@@ -1513,8 +1533,8 @@ int product(const Operand (&a)[2], const Operand (&b)[2], ProductArgs args, cons
     consider(2, 1, 4.0, 0.185, 64, cdiv(tiles(128, 64), sms));
     for (int split = 2; split <= 8 && split <= chunks && tiles(128, 128) * split <= sms; ++split) {
         const int clusters = clusters_at_once(split);
-        if (tiles(128, 128) <= clusters) consider(3, split, 7.2, 0.20, 0, 1);
-        if (tiles(128, 64) <= clusters) consider(4, split, 6.8, 0.18, 0, 1);
+        if (tiles(128, 128) <= clusters) consider(3, split, 7.3, 0.20, 0, 1);
+        if (tiles(128, 64) <= clusters) consider(4, split, 5.8, 0.18, 0, 1);
     }
     switch (which) {
         case 0: return launch_product<MODE, 2, 256, false, O, ACT>(a, b, args, name, s);
