@@ -547,14 +547,19 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, int limi
 }
 
 // Tile order: groups of 16 tile rows, columns inside a group, so that the CTAs
-// at work at one time read few operand rows (L2 hits). 8192 x 16384 x 4096
-// block: 1680 us with groups of 8, 1640 of 16, 1710 of 32.
+// at work at one time read few operand rows (L2 hits). 8192 x 16384 x 4096 block:
+// 1477 us with groups of 8, 1469 of 16, 1481 of 24; 8-bit product of 16384 x 16384 x
+// 4096: 732 / 717 / 717. The gradients sum over a long axis, along which all CTAs
+// move together and nothing stays in L2, so there the two operands' shares should
+// be alike: 3455 us with groups of 4, 3385 of 6, 3484 of 8, 3470 of 16.
+template <int MODE>
 __device__ __forceinline__ void tile_at(int i, int tiles_m, int tiles_n, int& m, int& n) {
-    const int group = 16 * tiles_n;
+    constexpr int kRows = MODE == kDx || MODE == kDw ? 6 : 16;
+    const int group = kRows * tiles_n;
     const int g = i / group, r = i - g * group;
-    const int h = min(16, tiles_m - g * 16);
+    const int h = min(kRows, tiles_m - g * kRows);
     n = r / h;
-    m = g * 16 + r - n * h;
+    m = g * kRows + r - n * h;
 }
 
 // A warp's 32 x 32 values (one row per lane) to a matrix at `to`, of which
@@ -669,7 +674,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
         bool ok = true;
         for (int tile = first; ok && tile < tiles; tile += step) {
             int mt, nt;
-            tile_at(tile, a.tiles_m, a.tiles_n, mt, nt);
+            tile_at<MODE>(tile, a.tiles_m, a.tiles_n, mt, nt);
             int pair = 0;
             if (MODE == kDw && mt >= a.tiles_m1) {
                 mt -= a.tiles_m1;
@@ -789,7 +794,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
         for (int tile = first; tile < tiles; tile += step, ++n) {
             const int buf = n & 1;
             int mt, nt;
-            tile_at(tile, a.tiles_m, a.tiles_n, mt, nt);
+            tile_at<MODE>(tile, a.tiles_m, a.tiles_n, mt, nt);
             int out = 0;
             if (MODE == kDw && mt >= a.tiles_m1) {
                 mt -= a.tiles_m1;
@@ -894,7 +899,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
     if constexpr (SPLIT) {
         // every CTA adds up its share of the tile's rows: a thread takes 4 columns of a row
         int mt, nt;
-        tile_at(first, a.tiles_m, a.tiles_n, mt, nt);
+        tile_at<MODE>(first, a.tiles_m, a.tiles_n, mt, nt);
         int out = 0;
         if (MODE == kDw && mt >= a.tiles_m1) {
             mt -= a.tiles_m1;
