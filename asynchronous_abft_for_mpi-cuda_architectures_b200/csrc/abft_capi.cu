@@ -82,7 +82,7 @@ extern "C" {
 
 const char* abft_last_error(void) { return g_last_error.c_str(); }
 
-int abft_version(void) { return 10000; }
+int abft_version(void) { return 10100; }
 
 size_t abft_ws_bytes(int M_b, int N_b, int K, int F, const int* counts, int max_iters) {
     if (M_b < 1 || N_b < 1 || K < 1 || F < 1 || !counts) return 0;

@@ -24,7 +24,6 @@ namespace {
 
 constexpr int kWaitLimit = 1 << 20;  // polls of the waits that follow one that ran out
 
-
 template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
@@ -423,7 +422,7 @@ __global__ void __launch_bounds__(ROW < 128 ? 128 : ROW, 1024 / (ROW < 128 ? 128
     }
 }
 
-// Column sums of an 8-bit weight: blocks of 256 rows, their sums added as
+// Column sums of an 8-bit weight: blocks of 512 rows, their sums added as
 // integers (the order does not matter). WIDE: 4 columns per load.
 template <bool WIDE>
 __global__ void __launch_bounds__(256) k_column_checksum(const int8_t* __restrict__ w, int64_t ldw, int N, int K,
@@ -431,17 +430,17 @@ __global__ void __launch_bounds__(256) k_column_checksum(const int8_t* __restric
     constexpr int kC = WIDE ? 4 : 1;
     const int64_t k = ((int64_t)blockIdx.x * 256 + threadIdx.x) * kC;
     if (k >= K) return;
-    const int last = min(N, ((int)blockIdx.y + 1) * 256);
+    const int first = (int)blockIdx.y * 512, last = min(N, first + 512);
     int sum[kC] = {};
     if (WIDE && k + kC <= K) {
 #pragma unroll 8
-        for (int n = blockIdx.y * 256; n < last; ++n) {
+        for (int n = first; n < last; ++n) {
             const int v = __ldg(reinterpret_cast<const int*>(w + n * ldw + k));
 #pragma unroll
             for (int i = 0; i < kC; ++i) sum[i] += static_cast<int8_t>(v >> (8 * i));
         }
     } else {
-        for (int n = blockIdx.y * 256; n < last; ++n)
+        for (int n = first; n < last; ++n)
 #pragma unroll
             for (int i = 0; i < kC; ++i)
                 if (k + i < K) sum[i] += w[n * ldw + k + i];
@@ -1240,6 +1239,16 @@ int bad(const char* msg) {
     return ABFT_ERR_ARG;
 }
 
+// Sizes whose tiles' indexes stay inside 32 bits.
+bool extents(int T, int N, int K) {
+    constexpr int kMost = ABFT_PRODUCT_MAX;
+    return T >= 0 && T <= kMost && N >= 1 && N <= kMost && K >= 1 && K <= kMost;
+}
+
+bool holds(const void* work, size_t bytes, size_t needed) {
+    return needed == 0 || (work && bytes >= needed && ((uintptr_t)work & 15) == 0);
+}
+
 int status(cudaError_t e, const char* what) { return e == cudaSuccess ? ABFT_OK : cuda_fail(e, what); }
 
 // Launches a kernel that may start up while the one before it ends.
@@ -1576,8 +1585,9 @@ extern "C" {
 
 int abft_quantize_rows(const void* dX, int64_t ldx, int type, int T, int K, int8_t* dQ, int64_t ldq, float* dScale,
                        const int32_t* dChecksum, int64_t* dExpect, void* stream) {
-    if (T < 0 || K < 1 || ldx < K || ldq < K || type < ABFT_TYPE_F32 || type > ABFT_TYPE_BF16)
-        return bad("abft_quantize_rows: bad argument (need T >= 0, K >= 1, ldx >= K, ldq >= K and an element type)");
+    if (!extents(T, 1, K) || ldx < K || ldq < K || type < ABFT_TYPE_F32 || type > ABFT_TYPE_BF16)
+        return bad("abft_quantize_rows: bad argument (need 0 <= T <= 2^30, 1 <= K <= 2^30, ldx >= K, ldq >= K and an "
+                   "element type)");
     if (T == 0) return ABFT_OK;
     if (!dX || !dQ || !dScale || (dChecksum != nullptr) != (dExpect != nullptr))
         return bad("abft_quantize_rows: bad argument (missing pointer, or one of dChecksum and dExpect alone)");
@@ -1590,12 +1600,12 @@ int abft_quantize_rows(const void* dX, int64_t ldx, int type, int T, int K, int8
 }
 
 int abft_column_checksum(const int8_t* dW, int64_t ldw, int N, int K, int32_t* dChecksum, void* stream) {
-    if (!dW || !dChecksum || N < 1 || N > ABFT_INT8_MAX_ROWS || K < 1 || ldw < K)
-        return bad("abft_column_checksum: bad argument (need pointers, 1 <= N <= 2^24, K >= 1, ldw >= K)");
+    if (!dW || !dChecksum || N < 1 || N > ABFT_INT8_MAX_ROWS || !extents(0, N, K) || ldw < K)
+        return bad("abft_column_checksum: bad argument (need pointers, 1 <= N <= 2^24, 1 <= K <= 2^30, ldw >= K)");
     cudaStream_t s = (cudaStream_t)stream;
     const cudaError_t e = cudaMemsetAsync(dChecksum, 0, sizeof(int32_t) * K, s);
     if (e != cudaSuccess) return cuda_fail(e, "abft_column_checksum");
-    const unsigned chunks = (unsigned)cdiv(N, 256);
+    const unsigned chunks = (unsigned)cdiv(N, 512);
     if (((uintptr_t)dW & 3) == 0 && (ldw & 3) == 0)
         k_column_checksum<true><<<dim3((unsigned)cdiv(K, 1024), chunks), 256, 0, s>>>(dW, ldw, N, K, dChecksum);
     else
@@ -1604,21 +1614,22 @@ int abft_column_checksum(const int8_t* dW, int64_t ldw, int N, int K, int32_t* d
 }
 
 size_t abft_int8_matmul_ws_bytes(const int8_t* dQ, int64_t ldq, const int8_t* dW, int64_t ldw, int T, int N, int K) {
-    if (T < 1 || N < 1 || K < 1) return 0;
+    if (T < 1 || !extents(T, N, K)) return 0;
     return Operand{dQ, ldq, T, K, 1}.bytes() + Operand{dW, ldw, N, K, 1}.bytes();
 }
 
 int abft_int8_matmul(const int8_t* dQ, int64_t ldq, const float* dQScale, const int8_t* dW, int64_t ldw,
                      const float* dWScale, int T, int N, int K, void* dY, int64_t ldy, int type,
                      const int64_t* dExpect, int64_t* dRowDiff, void* dWork, size_t work_bytes, void* stream) {
-    if (T < 0 || N < 1 || K < 1 || K > ABFT_INT8_MAX_K || ldq < K || ldw < K || ldy < N || type < ABFT_TYPE_F32 ||
+    if (!extents(T, N, K) || K > ABFT_INT8_MAX_K || ldq < K || ldw < K || ldy < N || type < ABFT_TYPE_F32 ||
         type > ABFT_TYPE_BF16)
-        return bad("abft_int8_matmul: bad argument (need T >= 0, N >= 1, 1 <= K <= 131071, ldq >= K, ldw >= K, "
-                   "ldy >= N and an element type)");
+        return bad("abft_int8_matmul: bad argument (need 0 <= T <= 2^30, 1 <= N <= 2^30, 1 <= K <= 131071, ldq >= K, "
+                   "ldw >= K, ldy >= N and an element type)");
     if (T == 0) return ABFT_OK;
     if (!dQ || !dQScale || !dW || !dWScale || !dY || (dExpect != nullptr) != (dRowDiff != nullptr))
         return bad("abft_int8_matmul: bad argument (missing pointer, or one of dExpect and dRowDiff alone)");
-    if (work_bytes < abft_int8_matmul_ws_bytes(dQ, ldq, dW, ldw, T, N, K)) return bad("abft_int8_matmul: workspace too small");
+    if (!holds(dWork, work_bytes, abft_int8_matmul_ws_bytes(dQ, ldq, dW, ldw, T, N, K)))
+        return bad("abft_int8_matmul: workspace missing, too small or not 16-byte aligned");
     cudaStream_t s = (cudaStream_t)stream;
     if (dExpect) {
         const cudaError_t e = launch_next(k_negate, dim3((unsigned)cdiv(T, 256)), 256, 0, s, dExpect, dRowDiff, T);
@@ -1647,7 +1658,7 @@ int abft_int8_matmul(const int8_t* dQ, int64_t ldq, const float* dQScale, const 
 
 size_t abft_gated_ffn_ws_bytes(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg, const void* dWUp,
                                int64_t ldwu, int T, int N, int K) {
-    if (T < 1 || N < 1 || K < 1) return 0;
+    if (T < 1 || !extents(T, N, K)) return 0;
     return Operand{dX, ldx, T, K, 2}.bytes() + Operand{dWGate, ldwg, N, K, 2}.bytes() +
            Operand{dWUp, ldwu, N, K, 2}.bytes();
 }
@@ -1655,16 +1666,16 @@ size_t abft_gated_ffn_ws_bytes(const void* dX, int64_t ldx, const void* dWGate, 
 int abft_gated_ffn(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg, const void* dWUp, int64_t ldwu,
                    int T, int N, int K, int type, int activation, void* dH, int64_t ldh, void* dG, int64_t ldg,
                    void* dU, int64_t ldu, void* dWork, size_t work_bytes, void* stream) {
-    if (T < 0 || N < 1 || K < 1 || ldx < K || ldwg < K || ldwu < K || ldh < N || (dG && ldg < N) || (dU && ldu < N) ||
+    if (!extents(T, N, K) || ldx < K || ldwg < K || ldwu < K || ldh < N || (dG && ldg < N) || (dU && ldu < N) ||
         (type != ABFT_TYPE_F16 && type != ABFT_TYPE_BF16) || activation < ABFT_ACT_SILU ||
         activation > ABFT_ACT_GELU_TANH)
-        return bad("abft_gated_ffn: bad argument (need T >= 0, N >= 1, K >= 1, pitches that hold a row, a 16-bit "
-                   "element type and an activation)");
+        return bad("abft_gated_ffn: bad argument (need 0 <= T <= 2^30, 1 <= N, K <= 2^30, pitches that hold a row, a "
+                   "16-bit element type and an activation)");
     if (T == 0) return ABFT_OK;
     if (!dX || !dWGate || !dWUp || !dH || (dG != nullptr) != (dU != nullptr))
         return bad("abft_gated_ffn: bad argument (missing pointer, or one of dG and dU alone)");
-    if (work_bytes < abft_gated_ffn_ws_bytes(dX, ldx, dWGate, ldwg, dWUp, ldwu, T, N, K))
-        return bad("abft_gated_ffn: workspace too small");
+    if (!holds(dWork, work_bytes, abft_gated_ffn_ws_bytes(dX, ldx, dWGate, ldwg, dWUp, ldwu, T, N, K)))
+        return bad("abft_gated_ffn: workspace missing, too small or not 16-byte aligned");
     cudaStream_t s = (cudaStream_t)stream;
     Operand x{dX, ldx, T, K, 2}, wg{dWGate, ldwg, N, K, 2}, wu{dWUp, ldwu, N, K, 2};
     char* work = (char*)dWork;
@@ -1689,7 +1700,7 @@ int abft_gated_ffn(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg
 
 size_t abft_gated_ffn_backward_ws_bytes(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg,
                                         const void* dWUp, int64_t ldwu, int T, int N, int K) {
-    if (T < 1 || N < 1 || K < 1) return 0;
+    if (T < 1 || !extents(T, N, K)) return 0;
     return 2 * grad_bytes(T, N) + abft_gated_ffn_ws_bytes(dX, ldx, dWGate, ldwg, dWUp, ldwu, T, N, K);
 }
 
@@ -1698,11 +1709,11 @@ int abft_gated_ffn_backward(const void* dDH, int64_t ldd, const void* dX, int64_
                             int64_t ldu, int T, int N, int K, int type, int activation, void* dDX, int64_t lddx,
                             void* dDWGate, int64_t lddwg, void* dDWUp, int64_t lddwu, void* dWork, size_t work_bytes,
                             void* stream) {
-    if (T < 0 || N < 1 || K < 1 || ldd < N || ldx < K || ldwg < K || ldwu < K || ldg < N || ldu < N || lddx < K ||
+    if (!extents(T, N, K) || ldd < N || ldx < K || ldwg < K || ldwu < K || ldg < N || ldu < N || lddx < K ||
         lddwg < K || lddwu < K || (type != ABFT_TYPE_F16 && type != ABFT_TYPE_BF16) || activation < ABFT_ACT_SILU ||
         activation > ABFT_ACT_GELU_TANH)
-        return bad("abft_gated_ffn_backward: bad argument (need T >= 0, N >= 1, K >= 1, pitches that hold a row, a "
-                   "16-bit element type and an activation)");
+        return bad("abft_gated_ffn_backward: bad argument (need 0 <= T <= 2^30, 1 <= N, K <= 2^30, pitches that hold "
+                   "a row, a 16-bit element type and an activation)");
     if (!dDWGate || !dDWUp) return bad("abft_gated_ffn_backward: bad argument (missing pointer)");
     cudaStream_t s = (cudaStream_t)stream;
     if (T == 0) {  // no token: the weights' gradients are empty sums
@@ -1712,8 +1723,8 @@ int abft_gated_ffn_backward(const void* dDH, int64_t ldd, const void* dX, int64_
     }
     if (!dDH || !dX || !dWGate || !dWUp || !dG || !dU || !dDX)
         return bad("abft_gated_ffn_backward: bad argument (missing pointer)");
-    if (!dWork || work_bytes < abft_gated_ffn_backward_ws_bytes(dX, ldx, dWGate, ldwg, dWUp, ldwu, T, N, K))
-        return bad("abft_gated_ffn_backward: workspace too small");
+    if (!holds(dWork, work_bytes, abft_gated_ffn_backward_ws_bytes(dX, ldx, dWGate, ldwg, dWUp, ldwu, T, N, K)))
+        return bad("abft_gated_ffn_backward: workspace missing, too small or not 16-byte aligned");
     const int64_t p = grad_pitch(N);
     char* work = (char*)dWork;
     const Operand dg{work, p, T, N, 2}, du{work + grad_bytes(T, N), p, T, N, 2};

@@ -9,14 +9,16 @@ one are kept from reuse until its work is done. Nothing is kept between calls,
 so they can be captured into CUDA graphs and issued on several streams.
 """
 import contextlib
+import ctypes
 
 import torch
 
-from ._lib import check, lib
+from ._lib import ABFT_ERR_CUDA, AbftError, check, lib
 
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 
+MAX_EXTENT = 1 << 30         # rows and columns of any matrix
 INT8_MAX_K = 131071          # 128 * 128 * K fits a 32-bit sum
 INT8_MAX_ROWS = 1 << 24      # 127 * N fits a 32-bit checksum
 
@@ -31,8 +33,8 @@ def _matrix(t, name, dtypes, rows=None, cols=None, device=None):
                          f"{'any' if cols is None else cols}")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
-    if c < 1 or r > 0x7fffffff or c > 0x7fffffff:
-        raise ValueError(f"{name} is {r} x {c}: rows of 1 to 2^31 - 1 elements are supported")
+    if c < 1 or r > MAX_EXTENT or c > MAX_EXTENT:
+        raise ValueError(f"{name} is {r} x {c}: rows of at least one element and extents up to 2^30 are supported")
     pitch, step = t.stride()
     if step != 1 and c > 1:
         raise ValueError(f"{name} must be row-major (stride 1 along a row)")
@@ -89,6 +91,19 @@ def _ptr(t):
 
 def _empty(rows, cols, pitch, dtype, device):
     return torch.empty_strided((rows, cols), (pitch, 1), dtype=dtype, device=device)
+
+
+def check_waits(device=None):
+    """Synchronous: raises AbftError if a wait inside a product kernel of the
+    device has run out since the last call (its kernels wait for their own
+    copies and matrix instructions, each wait with a limit); the results of the
+    calls since then are void."""
+    fault = ctypes.c_int()
+    with torch.cuda.device(device):
+        check(lib.abft_products_status(ctypes.byref(fault)), "abft_products_status")
+    if fault.value:
+        raise AbftError("products", ABFT_ERR_CUDA, "a wait inside a kernel did not end within the wait limit; the "
+                                                   "results since the last check are void")
 
 
 def quantize_rows(x, checksum=None, stream=None):

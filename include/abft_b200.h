@@ -48,6 +48,7 @@ extern "C" {
 #define ABFT_ACT_GELU 1      /* g * Phi(g)                                  */
 #define ABFT_ACT_GELU_TANH 2 /* its tanh approximation                      */
 
+#define ABFT_PRODUCT_MAX 1073741824 /* largest T, N and K of the products   */
 #define ABFT_INT8_MAX_K 131071      /* 128 * 128 * K fits a 32-bit sum      */
 #define ABFT_INT8_MAX_ROWS 16777216 /* 127 * N fits a 32-bit checksum       */
 
@@ -254,7 +255,8 @@ int abft_sgemm(void* cublas_handle, const float* dA, int lda, const float* dB, i
  * streams are independent as long as their outputs and workspaces are. The
  * current device must be the stream's. Matrices are row-major with a pitch in
  * elements; a weight is N x K (one row per output channel). Element types are
- * ABFT_TYPE_*. T may be 0. Inputs and outputs must not overlap.
+ * ABFT_TYPE_*. T may be 0; T, N and K are at most ABFT_PRODUCT_MAX. Inputs and
+ * outputs must not overlap.
  *
  * Workspaces: each *_ws_bytes function takes the inputs of its call and says
  * how many bytes of 16-byte aligned device memory that call needs as dWork

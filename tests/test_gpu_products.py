@@ -177,7 +177,9 @@ def test_column_checksum(N, K, abft):
 # ---------------------------------------------------------- 8-bit product ---
 
 @pytest.mark.parametrize("dtype", [torch.float32, *HALF])
-@pytest.mark.parametrize("T,N,K", SHAPES + [(40, 4096, 4096), (1, 5000, 8192), (1500, 2050, 96)])
+@pytest.mark.parametrize("T,N,K", SHAPES + [(40, 4096, 4096), (1, 5000, 8192), (1500, 2050, 96),
+                                            # pairs of SMs; K split over 8 and over 5 or 6 CTAs
+                                            (1000, 4096, 2060), (48, 520, 16000), (330, 500, 9000)])
 def test_int8_matmul(T, N, K, dtype, abft):
     g = gen(T + 3 * N + 5 * K)
     q = torch.randint(-128, 128, (T, K), generator=g, device="cuda", dtype=torch.int8)
@@ -262,7 +264,9 @@ def forward_def(x, wg, wu, kind, dtype):
 
 
 @pytest.mark.parametrize("dtype", HALF)
-@pytest.mark.parametrize("T,N,K", SHAPES + [(1, 4096, 4096), (24, 2048, 4096), (1100, 1300, 96)])
+@pytest.mark.parametrize("T,N,K", SHAPES + [(1, 4096, 4096), (24, 2048, 4096), (1100, 1300, 96),
+                                            # pairs of SMs; K split over the CTAs of a cluster
+                                            (1000, 2050, 1100), (48, 1000, 4100), (333, 500, 9000)])
 def test_gated_ffn(T, N, K, dtype, abft):
     kind = ACTS[(T + N) % 3]
     _, x, wg, wu = block(T + 2 * N + K, T, N, K, dtype)
@@ -309,7 +313,9 @@ def backward_def(dh, x, wg, wu, g, u, kind, dtype):
 
 
 @pytest.mark.parametrize("dtype", HALF)
-@pytest.mark.parametrize("T,N,K", SHAPES + [(4096, 136, 64), (700, 1000, 1300)])
+@pytest.mark.parametrize("T,N,K", SHAPES + [(4096, 136, 64), (700, 1000, 1300),
+                                            # pairs of SMs; N split; T split
+                                            (1000, 1100, 4100), (333, 4096, 1000), (9000, 130, 200)])
 def test_gated_ffn_backward(T, N, K, dtype, abft):
     kind = ACTS[(T + K) % 3]
     r, x, wg, wu = block(2 * T + N + K, T, N, K, dtype)
@@ -547,6 +553,148 @@ def test_outputs_keep_to_their_rows_and_columns(abft):
                 assert torch.equal(y, abft.products.int8_matmul(want[0], want[1], wq, ws, dtype=dtype))
                 assert untouched(Y, T, N)
                 nb and refuse_small_workspace(abft, args, s, ws, T, N, K, y, pad, code, work, nb, stream)
+
+
+FRESH = """
+import importlib, sys, torch
+sys.path.insert(0, {root!r})
+p = importlib.import_module({pkg!r}).products
+T, N, K = {shape}
+gen = torch.Generator(device="cuda").manual_seed(1)
+x, wg, wu, dh = (torch.randn(*s, generator=gen, device="cuda").bfloat16() for s in ((T, K), (N, K), (N, K), (T, N)))
+def run():
+    h, g, u = p.gated_ffn(x, wg, wu, save=True)
+    grads = p.gated_ffn_backward(dh, x, wg, wu, g, u)
+    wq, ws = p.quantize_rows(wg)
+    c = p.column_checksum(wq)
+    q, s, e = p.quantize_rows(x, checksum=c)
+    return (h, *grads, *p.int8_matmul(q, s, wq, ws, expect=e))
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    captured = run()
+graph.replay()
+torch.cuda.synchronize()
+for a, b in zip(captured, run()):
+    assert torch.equal(a, b)
+assert (captured[-1] == 0).all()
+p.check_waits()
+"""
+
+
+@pytest.mark.parametrize("shape", [(1, 300, 256), (40, 300, 256), (300, 2000, 256), (2100, 2560, 130)])
+def test_first_call_is_captured(shape):
+    """A process whose first call of every kernel is recorded into a graph."""
+    import os
+    import subprocess
+    import sys
+    from conftest import PKG_NAME, ROOT
+    r = subprocess.run([sys.executable, "-c", FRESH.format(root=ROOT, pkg=PKG_NAME, shape=shape)], capture_output=True,
+                       text=True, timeout=300, env=dict(os.environ))
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_offsets_past_32_bits(abft):
+    """Operands and results of more than 2^31 elements: the last rows as well as the first."""
+    p, g = abft.products, gen(4)
+    T, N, K = 70000, 40000, 32
+    q = torch.randint(-128, 128, (T, K), generator=g, device="cuda", dtype=torch.int8)
+    w = torch.randint(-128, 128, (N, K), generator=g, device="cuda", dtype=torch.int8)
+    one_t, one_n = torch.ones(T, device="cuda"), torch.ones(N, device="cuda")
+    e = (q.double() @ w.sum(0, dtype=torch.int32).double()).to(torch.int64)
+    y, diff = p.int8_matmul(q, one_t, w, one_n, dtype=torch.bfloat16, expect=e)
+    assert (diff == 0).all() and T * N > 2 ** 31
+    for rows in (slice(0, 200), slice(T - 200, T)):
+        assert torch.equal(y[rows], int_product(q[rows], w).bfloat16())
+    q8, s8, e8 = p.quantize_rows(y, checksum=torch.ones(N, dtype=torch.int32, device="cuda"))
+    for rows in (slice(0, 3), slice(T - 3, T)):
+        want_q, want_s = quantize_def(y[rows])
+        assert torch.equal(q8[rows], want_q) and torch.equal(s8[rows], want_s)
+        assert torch.equal(e8[rows], want_q.to(torch.int64).sum(1))
+    del y, q8
+    # few tokens and many channels on a wide pitch
+    wide = torch.empty(33000, 70000, dtype=torch.bfloat16, device="cuda")
+    wg, wu = wide[:, :64], wide[:, 64:128]
+    wg.normal_(generator=g)
+    wu.normal_(generator=g)
+    x = randn(g, 3, 64).bfloat16()
+    want = p.gated_ffn(x, wg.contiguous(), wu.contiguous(), save=True)
+    for a, b in zip(p.gated_ffn(x, wg, wu, save=True), want):
+        assert torch.equal(a, b)
+    x = randn(g, 140, 64).bfloat16()
+    h, gs, us = p.gated_ffn(x, wg, wu, save=True)
+    dh = randn(g, *h.shape).bfloat16()
+    for a, b in zip(p.gated_ffn_backward(dh, x, wg, wu, gs, us),
+                    p.gated_ffn_backward(dh, x, wg.contiguous(), wu.contiguous(), gs, us)):
+        assert torch.equal(a, b)
+
+
+def test_many_tokens_and_channels(abft):
+    """More rows than a grid's second dimension, in each place a row can stand."""
+    p = abft.products
+    for T, N, K in ((70000, 16, 24), (40, 140000, 16)):
+        r, x, wg, wu = block(5, T, N, K, torch.bfloat16)
+        wants = forward_def(x, wg, wu, "silu", torch.bfloat16)
+        got = p.gated_ffn(x, wg, wu, save=True)
+        for y, (want, tol) in zip(got, wants):
+            assert_near(y, want, tol)
+        dh = randn(r, T, N).bfloat16()
+        for y, (want, tol) in zip(p.gated_ffn_backward(dh, x, wg, wu, *got[1:]),
+                                  backward_def(dh, x, wg, wu, *got[1:], "silu", torch.bfloat16)):
+            assert_near(y, want, tol)
+    w = torch.full((1 << 24, 3), -128, dtype=torch.int8, device="cuda")
+    w[:, 1] = 127
+    assert p.column_checksum(w).tolist() == [-2 ** 31, 127 << 24, -2 ** 31]
+
+
+def test_streams_by_handle_and_freed_inputs(abft):
+    """A raw stream handle works like the stream; inputs dropped right after a call on another stream stay until it ran."""
+    p = abft.products
+    _, x, wg, wu = block(8, 600, 520, 264, torch.float16)
+    want = p.gated_ffn(x, wg, wu)
+    assert torch.equal(p.gated_ffn(x, wg, wu, stream=torch.cuda.current_stream().cuda_stream), want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    h = p.gated_ffn(x, wg, wu, stream=side.cuda_stream)
+    side.synchronize()
+    assert torch.equal(h, want)
+    got = []
+    for _ in range(20):
+        a, b, c = x.clone(), wg.clone(), wu.clone()
+        side.wait_stream(torch.cuda.current_stream())
+        got.append(p.gated_ffn(a, b, c, stream=side))
+        del a, b, c
+        torch.empty_like(x).fill_(7), torch.empty_like(wg).fill_(7), torch.empty_like(wu).fill_(7)
+    torch.cuda.synchronize()
+    for h in got:
+        assert torch.equal(h, want)
+    with pytest.raises(ValueError):
+        p.gated_ffn(x, wg.cpu(), wu)
+
+
+@pytest.mark.parametrize("T,N,K", [(40, 1024, 4096), (200, 300, 128), (3000, 4096, 64)])
+def test_waits_that_run_out(T, N, K, abft):
+    """With a limit of 0 every wait inside the kernels gives up at once: they
+    return, the status says so once, and the next calls are right again."""
+    p = abft.products
+    _, x, wg, wu = block(11, T, N, K, torch.bfloat16)
+    q, s = p.quantize_rows(x)
+    w, ws = p.quantize_rows(wg)
+    h, g, u = p.gated_ffn(x, wg, wu, save=True)
+    want = [t.clone() for t in (h, *p.gated_ffn_backward(h, x, wg, wu, g, u), p.int8_matmul(q, s, w, ws))]
+    p.check_waits()
+    before = abft.lib.abft_set_wait_limit(0)
+    try:
+        for call in (lambda: p.gated_ffn(x, wg, wu), lambda: p.gated_ffn_backward(h, x, wg, wu, g, u),
+                     lambda: p.int8_matmul(q, s, w, ws)):
+            call()
+            with pytest.raises(abft.AbftError, match="wait"):
+                p.check_waits()
+            p.check_waits()
+    finally:
+        abft.lib.abft_set_wait_limit(before)
+    for a, b in zip((p.gated_ffn(x, wg, wu), *p.gated_ffn_backward(h, x, wg, wu, g, u), p.int8_matmul(q, s, w, ws)), want):
+        assert torch.equal(a, b)
+    p.check_waits()
 
 
 def refuse_small_workspace(abft, args, s, ws, T, N, K, y, pad, code, work, nb, stream):

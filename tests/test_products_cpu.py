@@ -24,7 +24,8 @@ BACK = [FAKE, 8, FAKE, 64, FAKE, 64, FAKE, 64, FAKE, 8, FAKE, 8, 4, 8, 64, 2, 0,
 
 
 @pytest.mark.parametrize("place,value", [
-    (0, None), (1, 63), (2, 3), (2, -1), (3, -1), (4, 0), (5, None), (6, 63), (7, None),
+    (0, None), (1, 63), (2, 3), (2, -1), (3, -1), (3, (1 << 30) + 1), (4, 0), (4, (1 << 30) + 1), (5, None), (6, 63),
+    (7, None),
     (8, FAKE),  # a checksum without a place for the expected sums
     (9, FAKE),  # and the other way round
 ])
@@ -43,7 +44,8 @@ def test_column_checksum_refuses(abft, place, value):
 
 @pytest.mark.parametrize("place,value", [
     (0, None), (1, 63), (2, None), (3, None), (4, 63), (5, None), (6, -1), (7, 0), (8, 0), (8, 131072), (9, None),
-    (10, 7), (11, 3), (12, FAKE), (13, FAKE),
+    (10, 7), (11, 3), (12, FAKE), (13, FAKE), (6, (1 << 30) + 1), (7, (1 << 30) + 1),
+    (1, 65), (4, 65), (0, ctypes.c_void_p(264)), (3, ctypes.c_void_p(258)),  # operands to be copied, but no workspace
 ])
 def test_int8_matmul_refuses(abft, place, value):
     args = list(INT8)
@@ -53,7 +55,8 @@ def test_int8_matmul_refuses(abft, place, value):
 
 @pytest.mark.parametrize("place,value", [
     (0, None), (1, 63), (2, None), (3, 63), (4, None), (5, 63), (6, -1), (7, 0), (8, 0), (9, 0), (9, 3), (10, 3),
-    (10, -1), (11, None), (12, 7), (13, FAKE), (15, FAKE),
+    (10, -1), (11, None), (12, 7), (13, FAKE), (15, FAKE), (6, (1 << 30) + 1), (7, (1 << 30) + 1), (8, (1 << 30) + 1),
+    (1, 65), (3, 65), (5, 65), (2, ctypes.c_void_p(258)),  # operands to be copied, but no workspace
 ])
 def test_gated_ffn_refuses(abft, place, value):
     args = list(FFN)
@@ -64,7 +67,8 @@ def test_gated_ffn_refuses(abft, place, value):
 @pytest.mark.parametrize("place,value", [
     (0, None), (1, 7), (2, None), (3, 63), (4, None), (5, 63), (6, None), (7, 63), (8, None), (9, 7), (10, None),
     (11, 7), (12, -1), (13, 0), (14, 0), (15, 0), (16, 3), (17, None), (18, 63), (19, None), (20, 63), (21, None),
-    (22, 63), (23, None), (24, 1),
+    (22, 63), (23, None), (23, ctypes.c_void_p(264)), (24, 1), (12, (1 << 30) + 1), (13, (1 << 30) + 1),
+    (14, (1 << 30) + 1),
 ])
 def test_gated_ffn_backward_refuses(abft, place, value):
     args = list(BACK)
