@@ -647,8 +647,14 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
         *stop = 0;
         tensor::bar_init_fence();
     }
+    if constexpr (CG == 2) {  // tensor memory of a pair is taken, and given back, only while both CTAs run
+        __syncwarp();
+        tensor::cluster_arrive_relaxed();
+        tensor::cluster_wait();
+    }
     if (warp == 2) tensor::tmem_alloc<CG>(tensor::smem_u32(const_cast<uint32_t*>(tmem_slot)), S::kTmemCols);
     tensor::tc_fence_before();
+    __syncwarp();
     if constexpr (CG == 2) tensor::cluster_sync();
     else __syncthreads();
     if (SPLIT && warp < 4) tensor::cluster_arrive_relaxed();
@@ -774,6 +780,10 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
         if (rank == 0) tensor::mma_commit<CG>(drained);
         for (int i = 0; i < kWaitLimit && !tensor::bar_test(drained, 0); ++i) {
         }
+        // The other CTA's arrivals for the last sums travel behind its stores to global memory; they have to land before
+        // this CTA goes, since the barrier at the end does not wait for them.
+        for (int j = max(0, n - 2); CG == 2 && rank == 0 && ok && j < n; ++j)
+            ok = wait_for(sums_empty(j & 1), (j >> 1) & 1, a.limit, stop);
     } else if (warp >= 4) {
         // -------------------------------------------------- results ---
         // warps w and w + 4 take the same 32 rows, each half of the columns
@@ -886,7 +896,9 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
     if constexpr (SPLIT) {
         if (warp < 4) tensor::cluster_wait();
         tensor::cluster_sync();  // the partial sums are there
-    } else if constexpr (CG == 2) {  // the leader's instructions use both CTAs' memory; nothing waits for their stores
+    } else if constexpr (CG == 2) {
+        // The leader's instructions use both CTAs' memory. All that one CTA sends the other has landed before the receiver
+        // arrives here (its threads waited for it), so nobody waits for the stores to global memory.
         tensor::cluster_arrive_relaxed();
         tensor::cluster_wait();
     } else {
@@ -894,6 +906,10 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
     }
     tensor::tc_fence_after();
     if (warp == 2) tensor::tmem_free<CG>(tmem, S::kTmemCols);
+    if constexpr (CG == 2) {
+        tensor::cluster_arrive_relaxed();
+        tensor::cluster_wait();
+    }
 
     if constexpr (SPLIT) {
         // every CTA adds up its share of the tile's rows: a thread takes 4 columns of a row

@@ -671,6 +671,30 @@ def test_streams_by_handle_and_freed_inputs(abft):
         p.gated_ffn(x, wg.cpu(), wu)
 
 
+def test_many_launches_in_a_row(abft):
+    """Thousands of launches that follow each other without a pause, kernels of pairs of SMs among them: each starts up
+    while the one before it ends, and every result is the first one's. The host watches the time."""
+    import time
+    p, (T, N, K) = abft.products, (1024, 2048, 1024)
+    r, x, wg, wu = block(13, T, N, K, torch.bfloat16)
+    h, g, u = p.gated_ffn(x, wg, wu, save=True)
+    dh = randn(r, T, N).bfloat16()
+    w, ws = p.quantize_rows(wg)
+    q, s, e = p.quantize_rows(x, checksum=p.column_checksum(w))
+    want = [h, *p.gated_ffn_backward(dh, x, wg, wu, g, u), *p.int8_matmul(q, s, w, ws, expect=e)]
+    for _ in range(10):
+        for _ in range(200):
+            got = [p.gated_ffn(x, wg, wu), *p.gated_ffn_backward(dh, x, wg, wu, g, u),
+                   *p.int8_matmul(q, s, w, ws, expect=e)]
+        done, began = torch.cuda.Event(), time.monotonic()
+        done.record()
+        while not done.query():
+            assert time.monotonic() - began < 20
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    p.check_waits()
+
+
 @pytest.mark.parametrize("T,N,K", [(40, 1024, 4096), (200, 300, 128), (3000, 4096, 64)])
 def test_waits_that_run_out(T, N, K, abft):
     """With a limit of 0 every wait inside the kernels gives up at once: they
