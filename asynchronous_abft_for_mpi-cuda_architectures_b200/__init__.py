@@ -1,4 +1,4 @@
-"""B200-native asynchronous ABFT layer around SGEMM.
+"""B200-native asynchronous ABFT layer around SGEMM, and products of language models.
 
 The compute path is libabft_b200.so (hand-written sm_100a kernels, C ABI in
 include/abft_b200.h, C++ pipeline around cuBLAS SGEMM). This package is the
