@@ -32,7 +32,7 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
 // ------------------------------------------------------------ activations ---
 //
 //   silu       a = g s,                s = 1 / (1 + e^-g)      a' = s (1 + g (1 - s))
-//   gelu       a = g p,                p = erfc(-g/sqrt2) / 2    a' = p + g e^(-g^2/2) / sqrt(2 pi)
+//   gelu       a = g p,                p = Phi(g) (below)      a' = p + g e^(-g^2/2) / sqrt(2 pi)
 //   gelu_tanh  a = g t, t = s(2 c (g + b g^3)), c = sqrt(2/pi), b = 0.044715
 //                                      a' = t + 2 c g t (1 - t) (1 + 3 b g^2)
 //
@@ -46,10 +46,33 @@ constexpr float kTanhB = 0.044715f;
 constexpr float kSqrtHalf = 0.70710678118654752f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 
+// The normal distribution function. With z = |g| / sqrt2 and t = 1 / (1 + 0.4 z) its
+// tail is erfc(z) / 2 = t e^(f(t) - z^2) / 2, f(t) = ln(e^(z^2) erfc(z) / t); f is smooth
+// on (0, 1], and a polynomial of degree 8 fitted to it (least squares at 4000
+// Chebyshev nodes of 0 <= z <= 14, 64 bits) is off by 1e-7; evaluated in 32 bits the
+// tail is off by 4.2e-7 relative, plus what the exponential loses of its argument.
+// No branch and 18 instructions, where erfcf cost 3 to 4 us of results that are not
+// hidden behind products (1000 x 1536 x 1024 block: 13.5 us, 11.5 so).
+__device__ __forceinline__ float normal(float g) {
+    const float z = fabsf(g) * kSqrtHalf;
+    const float t = __fdividef(1.0f, fmaf(0.4f, z, 1.0f));
+    float f = -0.21217621862888336f;
+    f = fmaf(f, t, 0.9476717710494995f);
+    f = fmaf(f, t, -1.5340924263000488f);
+    f = fmaf(f, t, 1.0546685457229614f);
+    f = fmaf(f, t, -0.48204973340034485f);
+    f = fmaf(f, t, 0.3168873190879822f);
+    f = fmaf(f, t, 0.39554527401924133f);
+    f = fmaf(f, t, 1.0022913217544556f);
+    f = fmaf(f, t, -1.488745927810669f);
+    const float tail = 0.5f * t * __expf(fmaf(-z, z, f));
+    return g < 0.0f ? tail : 1.0f - tail;
+}
+
 template <int ACT>
 __device__ __forceinline__ float act(float g) {
     if constexpr (ACT == ABFT_ACT_SILU) return g * sigmoid(g);
-    if constexpr (ACT == ABFT_ACT_GELU) return 0.5f * g * erfcf(-g * kSqrtHalf);
+    if constexpr (ACT == ABFT_ACT_GELU) return g * normal(g);
     return g * sigmoid(kTanhC2 * (g + kTanhB * g * g * g));
 }
 
@@ -60,7 +83,7 @@ __device__ __forceinline__ void act_grad(float g, float& a, float& slope) {
         a = g * s;
         slope = s * (1.0f + g * (1.0f - s));
     } else if constexpr (ACT == ABFT_ACT_GELU) {
-        const float p = 0.5f * erfcf(-g * kSqrtHalf);
+        const float p = normal(g);
         a = g * p;
         slope = p + g * __expf(-0.5f * g * g) * kInvSqrt2Pi;
     } else {

@@ -1,6 +1,7 @@
 """Refusals of the language-model products: every bad argument is an error before any CUDA call."""
 import ctypes
 import inspect
+import math
 
 import pytest
 import torch
@@ -127,3 +128,29 @@ def test_rounding_rule_on_ties():
         for xi, qi in zip(x[::17], q[::17]):
             want = max(-127, min(127, round(Fraction(float(xi)) / Fraction(float(scale)))))
             assert int(qi) == want, (float(xi), float(scale))
+
+
+def test_normal_distribution_fit():
+    """The fitted tail of the normal distribution, restated in float32 from the kernel's source, against erfc: the fit is
+    off by 1.1e-7, nine multiply-adds and the reciprocal lose at most 2^-24 of terms below 1.6 each, and the exponent
+    (z^2 + f, rounded once) half a step of its size."""
+    import os
+    import re
+    import numpy as np
+    from conftest import PKG_NAME, ROOT
+    src = open(os.path.join(ROOT, PKG_NAME, "csrc", "abft_products.cu")).read()
+    body = src[src.index("float normal(float g)"):]
+    body = body[:body.index("\n}\n")]
+    f = np.float32
+    c = [f(v) for v in re.findall(r"float f = (-?[\d.]+)f;|fmaf\(f, t, (-?[\d.]+)f\)", body) for v in v if v]
+    assert len(c) == 9
+    z = np.linspace(0, 9.2, 40001).astype(f)
+    t = (f(1) / (f(0.4) * z + f(1))).astype(f)
+    p = np.full_like(t, c[0])
+    for v in c[1:]:
+        p = (p.astype(np.float64) * t + v).astype(f)
+    arg = (p.astype(np.float64) - z.astype(np.float64) ** 2).astype(f)
+    got = t.astype(np.float64) * np.exp(arg.astype(np.float64))
+    want = np.array([math.erfc(float(v)) for v in z])
+    tol = 1.1e-7 + 10 * 1.6 * 2.0 ** -24 + np.abs(arg) * 2.0 ** -24
+    assert (np.abs(got / want - 1) <= tol).all()
