@@ -1549,7 +1549,8 @@ int clusters_at_once(int split) {
 
 // Tile and split by an estimate in us: a start and an end, and for every round of
 // tiles its chunks of 128 bytes of K or its results on their way out, whichever
-// is longer:
+// is longer (kGate counts as if g or u were kept too, whether or not, so that h
+// does not depend on it):
 //
 //                       start + end   a chunk (alone / all SMs busy)   32 x 32 results of a warp
 //   pair of SMs, 256        5.2        0.30  (0.28 / 0.31)              4 x 0.45
@@ -1569,11 +1570,10 @@ int product(const Operand (&a)[2], const Operand (&b)[2], ProductArgs args, cons
         return (MODE == kDw ? 2 : 1) * cdiv(args.rows, rows) * cdiv(args.cols, MODE == kGate ? columns / 2 : columns);
     };
     const int sms = sm_count();
-    const int outputs = args.c[1] && MODE == kGate ? 3 : MODE == kGate ? 1 : 2;  // in halves of a tile
     double best = 1e30;
     int which = 0;
     auto consider = [&](int i, int split, double ends, double chunk, int columns, int64_t rounds) {
-        const double round = std::max(chunk * (double)cdiv(chunks, split), 0.45 / 128 * columns * outputs);
+        const double round = std::max(chunk * (double)cdiv(chunks, split), 0.45 / 64 * columns);
         const double us = ends + round * (double)rounds;
         if (us < best) {
             best = us;

@@ -6,7 +6,8 @@ stream) and returns immediately; matrices are row-major torch CUDA tensors
 allocated on that stream; the rows of an output whose width is not a multiple of
 8 (of q: 16) lie on a pitch that is; inputs handed to a stream that is not the current
 one are kept from reuse until its work is done. Nothing is kept between calls,
-so they can be captured into CUDA graphs and issued on several streams.
+so they can be captured into CUDA graphs and issued on several streams. No
+autograd graph is recorded: gated_ffn_backward gives the gradients.
 """
 import contextlib
 import ctypes
