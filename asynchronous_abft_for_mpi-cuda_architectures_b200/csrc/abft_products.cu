@@ -445,15 +445,15 @@ __global__ void __launch_bounds__(ROW < 128 ? 128 : ROW, 1024 / (ROW < 128 ? 128
     }
 }
 
-// Column sums of an 8-bit weight: blocks of 512 rows, their sums added as
+// Column sums of an 8-bit weight: blocks of `rows` rows, their sums added as
 // integers (the order does not matter). WIDE: 4 columns per load.
 template <bool WIDE>
 __global__ void __launch_bounds__(256) k_column_checksum(const int8_t* __restrict__ w, int64_t ldw, int N, int K,
-                                                         int32_t* __restrict__ checksum) {
+                                                         int rows, int32_t* __restrict__ checksum) {
     constexpr int kC = WIDE ? 4 : 1;
     const int64_t k = ((int64_t)blockIdx.x * 256 + threadIdx.x) * kC;
     if (k >= K) return;
-    const int first = (int)blockIdx.y * 512, last = min(N, first + 512);
+    const int first = (int)blockIdx.y * rows, last = min(N, first + rows);
     int sum[kC] = {};
     if (WIDE && k + kC <= K) {
 #pragma unroll 8
@@ -629,7 +629,8 @@ __device__ __forceinline__ void store_block(char* mine, O* to, int64_t ld, int r
 }
 
 template <int MODE, int CG, int BN, bool SPLIT, typename O, int ACT>
-__global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_constant__ ProductMaps maps, const ProductArgs a) {
+__global__ void __launch_bounds__(kProductThreads, 1)
+    k_product(const __grid_constant__ ProductMaps maps, const ProductArgs a) {
     using S = Shape<MODE, CG, BN, SPLIT, O>;
     static_assert(!SPLIT || (128 + 8) * S::kPart * 4 <= S::kOut, "the partial sums fit the stages");
     static_assert(!SPLIT || CG == 1, "a split tile is one CTA wide");
@@ -875,7 +876,8 @@ __global__ void __launch_bounds__(kProductThreads, 1) k_product(const __grid_con
                 float v[32];
                 if constexpr (SPLIT) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) tensor::store_cluster(part + (j + i) * 4, r[i], r[i + 1], r[i + 2], r[i + 3]);
+                    for (int i = 0; i < 32; i += 4)
+                        tensor::store_cluster(part + (j + i) * 4, r[i], r[i + 1], r[i + 2], r[i + 3]);
                 } else if constexpr (MODE == kInt8) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
@@ -1644,11 +1646,12 @@ int abft_column_checksum(const int8_t* dW, int64_t ldw, int N, int K, int32_t* d
     cudaStream_t s = (cudaStream_t)stream;
     const cudaError_t e = cudaMemsetAsync(dChecksum, 0, sizeof(int32_t) * K, s);
     if (e != cudaSuccess) return cuda_fail(e, "abft_column_checksum");
-    const unsigned chunks = (unsigned)cdiv(N, 512);
+    const int rows = std::max(256, (int)cdiv(N, 65535));  // a grid has 65535 blocks in y
+    const unsigned chunks = (unsigned)cdiv(N, rows);
     if (((uintptr_t)dW & 3) == 0 && (ldw & 3) == 0)
-        k_column_checksum<true><<<dim3((unsigned)cdiv(K, 1024), chunks), 256, 0, s>>>(dW, ldw, N, K, dChecksum);
+        k_column_checksum<true><<<dim3((unsigned)cdiv(K, 1024), chunks), 256, 0, s>>>(dW, ldw, N, K, rows, dChecksum);
     else
-        k_column_checksum<false><<<dim3((unsigned)cdiv(K, 256), chunks), 256, 0, s>>>(dW, ldw, N, K, dChecksum);
+        k_column_checksum<false><<<dim3((unsigned)cdiv(K, 256), chunks), 256, 0, s>>>(dW, ldw, N, K, rows, dChecksum);
     return status(cudaGetLastError(), "abft_column_checksum");
 }
 
