@@ -802,7 +802,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         }
         // instructions in flight still read shared and write tensor memory, in both CTAs of a pair
         if (rank == 0) tensor::mma_commit<CG>(drained);
-        for (int i = 0; i < kWaitLimit && !tensor::bar_test(drained, 0); ++i) {
+        // (CTA 1 waits here from its start on: up to about a minute of kernel, unless a wait has run out)
+        for (int i = 0; !tensor::bar_test(drained, 0) && (i < kWaitLimit || (i < 64 * kWaitLimit && !*stop)); ++i) {
         }
         // The other CTA's arrivals for the last sums travel behind its stores to global memory; they have to land before
         // this CTA goes, since the barrier at the end does not wait for them.
