@@ -1388,13 +1388,14 @@ cudaError_t quantize(QuantArgs a, cudaStream_t s) {
         constexpr int kRow = decltype(row)::value, kU = decltype(u)::value, kBlock = kRow < 128 ? 128 : kRow;
         const int smem = decltype(check)::value && kU > 0 ? (int)cdiv(a.K, 8) * 32 : 0;
         auto kernel = k_quantize_rows<T, kRow, kU, decltype(check)::value>;
-        if (smem > 48 * 1024)
+        // a block has 48 KB unless more is asked for; the kernel's own variables (less than 1 KB) count too
+        if (smem > 47 * 1024)
             result = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
         int64_t blocks = cdiv(a.T, kBlock / kRow);
         if (blocks > sm_count()) {  // as many as are resident at a time, each with the same number of rows
             int resident = 1;
             if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kBlock, smem) != cudaSuccess) resident = 1;
-            blocks = std::min<int64_t>(blocks, (int64_t)sm_count() * resident);
+            blocks = std::min<int64_t>(blocks, (int64_t)sm_count() * std::max(resident, 1));
         }
         if (result == cudaSuccess) result = launch_next(kernel, dim3((unsigned)blocks), kBlock, smem, s, a);
     };

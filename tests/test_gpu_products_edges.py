@@ -1,0 +1,56 @@
+"""The language-model products where calls meet limits: of shared memory, of views, of streams and threads, of a type's range.
+
+Tolerances as in test_gpu_products: half a step for every rounding.
+"""
+import math
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from conftest import PKG_NAME, ROOT
+from test_gpu_products import HALF, assert_near, block, gen, half_step, int_product, quantize_def, randn, same
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------- checksums that fill shared memory ---
+
+def expected_sums(q, c):
+    return (q.cpu().to(torch.int64) * c.cpu().to(torch.int64)).sum(1).cuda()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, *HALF])
+@pytest.mark.parametrize("K", [8193, 12192, 12193, 12288, 12289, 16384, 16385])
+@pytest.mark.parametrize("T", [1, 149, 400])
+def test_wide_rows_with_a_checksum(T, K, dtype, abft):
+    g = gen(T + K)
+    x = randn(g, T, K).to(dtype)
+    c = torch.randint(-2 ** 31, 2 ** 31 - 1, (K,), generator=g, device="cuda", dtype=torch.int32)
+    q, scale, expect = abft.products.quantize_rows(x, checksum=c)
+    want_q, want_s = quantize_def(x)
+    assert torch.equal(q, want_q) and torch.equal(scale, want_s)
+    assert torch.equal(expect, expected_sums(want_q, c))
+
+
+FIRST = """
+import importlib, sys, torch
+sys.path.insert(0, {root!r})
+p = importlib.import_module({pkg!r}).products
+for dtype in (torch.float32, torch.float16, torch.bfloat16):
+    x = torch.randn({T}, 12288, device="cuda").to(dtype)
+    c = torch.randint(-20000, 20000, (12288,), device="cuda", dtype=torch.int32)
+    q, scale, expect = p.quantize_rows(x, checksum=c)
+    assert torch.equal(expect.cpu(), (q.cpu().long() * c.cpu().long()).sum(1))
+    assert torch.equal(q, p.quantize_rows(x)[0])
+"""
+
+
+@pytest.mark.parametrize("T", [1, 400])
+def test_wide_rows_with_a_checksum_come_first(T):
+    """A process whose first rows have checksums of just 48 KB: no wider call has raised the kernel's limit before."""
+    r = subprocess.run([sys.executable, "-c", FIRST.format(root=ROOT, pkg=PKG_NAME, T=T)], capture_output=True, text=True,
+                       timeout=300, env=dict(os.environ))
+    assert r.returncode == 0, r.stderr[-2000:]
