@@ -1321,6 +1321,9 @@ struct Operand {
     // on a pitch of 2016 bytes, 11.3 on 2048)
     int64_t packed_pitch() const { return cdiv((int64_t)cols * size, 128) * 128 / size; }
     size_t bytes() const { return direct() ? 0 : ((size_t)rows * packed_pitch() * size + 255) & ~(size_t)255; }
+    bool same(const Operand& o) const {
+        return p == o.p && ld == o.ld && rows == o.rows && cols == o.cols && size == o.size;
+    }
 
     // Boxes of 128 bytes x box_rows.
     bool map(CUtensorMap* m, int box_rows) const {
@@ -1434,8 +1437,8 @@ int launch_product(const Operand (&a)[2], const Operand (&b)[2], ProductArgs arg
     bool made = a[0].map(&maps.a[0], a_box) && b[0].map(&maps.b[0], b_box);
     maps.a[1] = maps.a[0];
     maps.b[1] = maps.b[0];
-    if (made && a[1].p != a[0].p) made = a[1].map(&maps.a[1], a_box);
-    if (made && b[1].p != b[0].p) made = b[1].map(&maps.b[1], b_box);
+    if (made && !a[1].same(a[0])) made = a[1].map(&maps.a[1], a_box);
+    if (made && !b[1].same(b[0])) made = b[1].map(&maps.b[1], b_box);
     if (!made) {
         set_error(std::string(name) + ": a tensor map could not be made");
         return ABFT_ERR_CUDA;

@@ -54,3 +54,24 @@ def test_wide_rows_with_a_checksum_come_first(T):
     r = subprocess.run([sys.executable, "-c", FIRST.format(root=ROOT, pkg=PKG_NAME, T=T)], capture_output=True, text=True,
                        timeout=300, env=dict(os.environ))
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+# ------------------------------------------------------ views of one buffer ---
+
+@pytest.mark.parametrize("T", [4, 40, 200, 1000])
+@pytest.mark.parametrize("order", [0, 1])
+def test_weights_that_start_at_one_place(T, order, abft):
+    """Two weights with the same first row and different pitches (every row and every second one of a buffer)."""
+    N, K = 264, 136
+    g = gen(T)
+    rows = (randn(g, 2 * N, K) / math.sqrt(K)).bfloat16()
+    views = rows[:N], rows[::2]
+    wg, wu = views[order], views[1 - order]
+    x, dh = randn(g, T, K).bfloat16(), randn(g, T, N).bfloat16()
+    p = abft.products
+    got = p.gated_ffn(x, wg, wu, save=True)
+    want = p.gated_ffn(x, wg.contiguous(), wu.contiguous(), save=True)
+    got += p.gated_ffn_backward(dh, x, wg, wu, *want[1:])
+    want += p.gated_ffn_backward(dh, x, wg.contiguous(), wu.contiguous(), *want[1:])
+    for a, b, name in zip(got, want, ("h", "g", "u", "dx", "dw_gate", "dw_up")):
+        assert torch.equal(a, b), name
