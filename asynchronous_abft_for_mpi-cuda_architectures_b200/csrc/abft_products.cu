@@ -1811,7 +1811,8 @@ int abft_products_status(int* fault) {
     if (!fault) return bad("abft_products_status: fault is NULL");
     unsigned f = 0;
     const unsigned none = 0;
-    cudaError_t e = cudaMemcpyFromSymbol(&f, g_fault, sizeof(f));
+    cudaError_t e = cudaDeviceSynchronize();  // a copy alone does not wait for streams made not to wait for it
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&f, g_fault, sizeof(f));
     if (e == cudaSuccess && f) e = cudaMemcpyToSymbol(g_fault, &none, sizeof(none));
     if (e != cudaSuccess) return cuda_fail(e, "abft_products_status");
     *fault = (int)f;

@@ -95,10 +95,11 @@ def _empty(rows, cols, pitch, dtype, device):
 
 
 def check_waits(device=None):
-    """Synchronous: raises AbftError if a wait inside a product kernel of the
-    device has run out since the last call (its kernels wait for their own
-    copies and matrix instructions, each wait with a limit); the results of the
-    calls since then are void."""
+    """Synchronous: waits for all work on the device, its other streams' too, and
+    raises AbftError if a wait inside a product kernel has run out since the last
+    call (its kernels wait for their own copies and matrix instructions, each wait
+    with a limit); the results of the calls since then are void. Not to be called
+    while a stream is being captured."""
     fault = ctypes.c_int()
     with torch.cuda.device(device):
         check(lib.abft_products_status(ctypes.byref(fault)), "abft_products_status")

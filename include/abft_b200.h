@@ -266,7 +266,8 @@ int abft_sgemm(void* cublas_handle, const float* dA, int lda, const float* dB, i
  * they are copied into the workspace first.
  * ---------------------------------------------------------------------- */
 
-/* Synchronous: whether a wait inside a product kernel of the current device has
+/* Synchronous: waits for all work on the current device (not to be called while
+ * a stream is being captured), then says whether a wait inside a product kernel has
  * run out since the last call (*fault = 1, then cleared). The kernels wait for
  * their own copies and matrix instructions only, each wait with a limit
  * (abft_set_wait_limit); after one that runs out they finish what is in

@@ -75,3 +75,33 @@ def test_weights_that_start_at_one_place(T, order, abft):
     want += p.gated_ffn_backward(dh, x, wg.contiguous(), wu.contiguous(), *want[1:])
     for a, b, name in zip(got, want, ("h", "g", "u", "dx", "dw_gate", "dw_up")):
         assert torch.equal(a, b), name
+
+
+# ------------------------------------------------- the status of the waits ---
+
+def run_out(abft, call):
+    """Makes every wait of the kernels that `call` launches give up at once."""
+    before = abft.lib.abft_set_wait_limit(0)
+    try:
+        call()
+    finally:
+        abft.lib.abft_set_wait_limit(before)
+
+
+def test_status_waits_for_other_streams(abft):
+    """A check right after a call on a side stream, whose kernel has not begun by then."""
+    p = abft.products
+    _, x, wg, wu = block(31, 200, 300, 128, torch.bfloat16)
+    want = p.gated_ffn(x, wg, wu)
+    p.check_waits()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)  # 0.2 s
+    run_out(abft, lambda: p.gated_ffn(x, wg, wu, stream=side))
+    with pytest.raises(abft.AbftError, match="wait"):
+        p.check_waits()
+    p.check_waits()
+    h = p.gated_ffn(x, wg, wu, stream=side)
+    p.check_waits()
+    assert torch.equal(h, want)
