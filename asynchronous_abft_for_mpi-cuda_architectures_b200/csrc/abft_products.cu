@@ -525,8 +525,9 @@ struct ProductMaps {
     CUtensorMap a[2], b[2];
 };
 
-// Waits that ran out since the last abft_products_status, any product kernel of the device.
-__device__ unsigned g_fault;
+// Waits that ran out in any product kernel of the device. It only grows: each host
+// thread compares it with what it was told last, so none takes a fault from another.
+__device__ unsigned g_faults;
 
 constexpr int kProductThreads = 384;  // copies, matrix instructions, 2 idle warps (one holds tensor memory), 8 for results
 
@@ -563,7 +564,7 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, int limi
     }
     if (!*stop) {
         *stop = 1;
-        atomicExch(&g_fault, 1u);
+        atomicAdd(&g_faults, 1u);
     }
     return false;
 }
@@ -1809,13 +1810,15 @@ int abft_gated_ffn_backward(const void* dDH, int64_t ldd, const void* dX, int64_
 
 int abft_products_status(int* fault) {
     if (!fault) return bad("abft_products_status: fault is NULL");
-    unsigned f = 0;
-    const unsigned none = 0;
-    cudaError_t e = cudaDeviceSynchronize();  // a copy alone does not wait for streams made not to wait for it
-    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&f, g_fault, sizeof(f));
-    if (e == cudaSuccess && f) e = cudaMemcpyToSymbol(g_fault, &none, sizeof(none));
+    static thread_local unsigned told[64];  // of each device
+    int dev = 0;
+    unsigned now = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();  // a copy alone does not wait for streams made not to wait for it
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&now, g_faults, sizeof(now));
     if (e != cudaSuccess) return cuda_fail(e, "abft_products_status");
-    *fault = (int)f;
+    *fault = now != (dev < 64 ? told[dev] : 0);
+    if (dev < 64) told[dev] = now;
     return ABFT_OK;
 }
 

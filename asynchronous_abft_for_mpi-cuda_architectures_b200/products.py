@@ -96,10 +96,11 @@ def _empty(rows, cols, pitch, dtype, device):
 
 def check_waits(device=None):
     """Synchronous: waits for all work on the device, its other streams' too, and
-    raises AbftError if a wait inside a product kernel has run out since the last
-    call (its kernels wait for their own copies and matrix instructions, each wait
-    with a limit); the results of the calls since then are void. Not to be called
-    while a stream is being captured."""
+    raises AbftError if a wait inside a product kernel has run out since this host
+    thread's last check (its first: since the library was loaded). The kernels wait
+    for their own copies and matrix instructions, each wait with a limit; after one
+    that ran out, the results of the calls since the last check are void. Not to be
+    called while a stream is being captured."""
     fault = ctypes.c_int()
     with torch.cuda.device(device):
         check(lib.abft_products_status(ctypes.byref(fault)), "abft_products_status")

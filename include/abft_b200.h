@@ -268,10 +268,12 @@ int abft_sgemm(void* cublas_handle, const float* dA, int lda, const float* dB, i
 
 /* Synchronous: waits for all work on the current device (not to be called while
  * a stream is being captured), then says whether a wait inside a product kernel has
- * run out since the last call (*fault = 1, then cleared). The kernels wait for
- * their own copies and matrix instructions only, each wait with a limit
- * (abft_set_wait_limit); after one that runs out they finish what is in
- * flight, return, and the results of calls since the last status are void. */
+ * run out since the calling host thread's last call (*fault = 1); its first call
+ * tells of the time since the library was loaded. What one thread has been told
+ * does not take it from another. The kernels wait for their own copies and matrix
+ * instructions only, each wait with a limit (abft_set_wait_limit); after one that
+ * runs out they finish what is in flight, return, and the results of calls since the
+ * last status are void. */
 int abft_products_status(int* fault);
 
 /* Rows to 8-bit integers: dScale[t] = fl32(max_k |x[t,k]| / 127) and

@@ -105,3 +105,25 @@ def test_status_waits_for_other_streams(abft):
     h = p.gated_ffn(x, wg, wu, stream=side)
     p.check_waits()
     assert torch.equal(h, want)
+
+
+def test_a_thread_is_told_of_a_fault_that_another_has_seen(abft):
+    from concurrent.futures import ThreadPoolExecutor
+    p = abft.products
+    _, x, wg, wu = block(32, 200, 300, 128, torch.bfloat16)
+
+    def told():
+        try:
+            p.check_waits(x.device)
+        except abft.AbftError:
+            return True
+        return False
+    with ThreadPoolExecutor(1) as other:
+        told(), other.submit(told).result()
+        assert not told() and not other.submit(told).result()
+        run_out(abft, lambda: p.gated_ffn(x, wg, wu))
+        assert other.submit(told).result() and told()
+        assert not other.submit(told).result() and not told()
+        run_out(abft, lambda: p.gated_ffn(x, wg, wu))
+        assert told() and other.submit(told).result()
+        assert not told() and not other.submit(told).result()
