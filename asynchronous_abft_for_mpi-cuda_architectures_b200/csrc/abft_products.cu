@@ -553,6 +553,22 @@ struct Shape {
     static constexpr int kTmemCols = 2 * BN;
 };
 
+// sum * row * column in this order: three roundings in 32 bits (in 64 bits each result
+// would cost two conversions, which the results' warps have no time for in short
+// products). Only sum * row could overflow where the result does not: a row's scale
+// from 2^64 on is used 2^32 times smaller, which keeps that product (sum < 2^31) below
+// 2^127 and above 2^32, and the result is taken back by 2^32. The other end needs
+// nothing: a whole number times a subnormal scale loses no bits.
+struct RowScale {
+    float scale, back;
+
+    explicit __device__ __forceinline__ RowScale(float s)
+        : scale(s >= 0x1p64f ? s * 0x1p-32f : s), back(s >= 0x1p64f ? 0x1p32f : 1.0f) {}
+    __device__ __forceinline__ float times(int sum, float column) const {
+        return static_cast<float>(sum) * scale * column * back;
+    }
+};
+
 // SPLIT: rows of the largest share of a tile, at most.
 __device__ __forceinline__ int share_rows(int split) { return 128 / split + (128 % split != 0); }
 
@@ -839,9 +855,9 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             const int rows = a.rows - m0;
             const int n0 = nt * S::kCols;
             long long total = 0;
-            float rs = 0.0f;
+            RowScale rs(0.0f);
             if constexpr (MODE == kInt8 && !SPLIT) {
-                if (lane < rows) rs = a.row_scale[m0 + lane];
+                if (lane < rows) rs = RowScale(a.row_scale[m0 + lane]);
                 __syncwarp();
                 for (int j = j0 + lane; j < j1; j += 32) sc[j - j0] = n0 + j < a.cols ? a.col_scale[n0 + j] : 0.0f;
                 __syncwarp();
@@ -889,7 +905,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
                         for (int k = 0; k < 4; ++k) {
                             const int sum = static_cast<int>(r[i + k]);
                             total += sum;
-                            v[i + k] = static_cast<float>(sum) * rs * scale[k];
+                            v[i + k] = rs.times(sum, scale[k]);
                         }
                     }
                     put(0, j, v);
@@ -990,10 +1006,9 @@ __global__ void __launch_bounds__(kProductThreads, 1)
                 int v[4] = {};
                 sum(r, c, v);
                 float y[4];
+                const RowScale rs(live ? a.row_scale[m] : 0.0f);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    y[i] = static_cast<float>(v[i]) * (live ? a.row_scale[m] : 0.0f) *
-                           (n0 + c + i < a.cols ? a.col_scale[n0 + c + i] : 0.0f);
+                for (int i = 0; i < 4; ++i) y[i] = rs.times(v[i], n0 + c + i < a.cols ? a.col_scale[n0 + c + i] : 0.0f);
                 if (live) put(0, m, c, y);
                 if (a.rowdiff) {
                     long long total = (long long)v[0] + v[1] + v[2] + v[3];
@@ -1159,10 +1174,10 @@ __global__ void __launch_bounds__(256, 2) k_few(const FewArgs a) {
                 s1 += static_cast<int>(part[first + w][i + 2][from]);
             }
             const bool in0 = tok < a.T && n < a.N, in1 = tok < a.T && n + 8 < a.N;
-            const float rs = tok < a.T ? a.row_scale[tok] : 0.0f;
+            const RowScale rs(tok < a.T ? a.row_scale[tok] : 0.0f);
             O* row = reinterpret_cast<O*>(a.c[0]) + tok * a.ld[0];
-            if (in0) row[n] = from_f32<O>(static_cast<float>(s0) * rs * a.col_scale[n]);
-            if (in1) row[n + 8] = from_f32<O>(static_cast<float>(s1) * rs * a.col_scale[n + 8]);
+            if (in0) row[n] = from_f32<O>(rs.times(s0, a.col_scale[n]));
+            if (in1) row[n + 8] = from_f32<O>(rs.times(s1, a.col_scale[n + 8]));
             if (a.rowdiff) {
                 long long sum = (in0 ? (long long)s0 : 0) + (in1 ? (long long)s1 : 0);
                 for (int o = 4; o; o >>= 1) sum += __shfl_down_sync(~0u, sum, o, 8);

@@ -158,7 +158,8 @@ def int8_matmul(q, q_scale, w, w_scale, dtype=torch.bfloat16, expect=None, strea
     """y[t, n] = (sum_k q[t, k] * w[n, k]) * q_scale[t] * w_scale[n].
 
     q (T x K) and w (N x K) are int8 (K <= 131071), the scales float32; the sums
-    are exact, y has the given dtype (float32, float16, bfloat16).
+    are exact and scaled in 32 bits, in this order (three roundings, and no overflow
+    unless the result does), y has the given dtype (float32, float16, bfloat16).
 
     expect (from quantize_rows) verifies the product while it is computed:
     returns (y, rowdiff) with rowdiff[t] = sum_n sum_k q[t, k] * w[n, k] -

@@ -296,7 +296,8 @@ int abft_column_checksum(const int8_t* dW, int64_t ldw, int N, int K, int32_t* d
 
 /* y[t,n] = (sum_k q[t,k] * w[n,k]) * dQScale[t] * dWScale[n], the sum exact in
  * 32 bits (K <= ABFT_INT8_MAX_K), the scales applied in 32-bit floating point
- * in this order, rounded once to the type of dY.
+ * in this order (the sum and both products are rounded, none overflows unless the
+ * result does), rounded once to the type of dY.
  * With dExpect[T] (from abft_quantize_rows) the product is verified while it
  * is computed: dRowDiff[t] = sum_n sum_k q[t,k] * w[n,k] - dExpect[t], taken
  * from the integer sums themselves. It is exactly 0 for every sound row: there

@@ -127,3 +127,40 @@ def test_a_thread_is_told_of_a_fault_that_another_has_seen(abft):
         run_out(abft, lambda: p.gated_ffn(x, wg, wu))
         assert told() and other.submit(told).result()
         assert not told() and not other.submit(told).result()
+
+
+# ------------------------------------------------------ the types' ranges ---
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,N,K", [(3, 40, 520), (30, 72, 4096), (40, 72, 4096), (300, 300, 256), (1100, 2100, 128)])
+def test_scales_over_the_whole_range(T, N, K, dtype, abft):
+    """Row and channel scales from the smallest subnormal number to the largest: a result is right wherever it is a number
+    of the type, however large the sum times the row's scale is."""
+    g = gen(T + N + K)
+    q = torch.randint(-127, 128, (T, K), generator=g, device="cuda", dtype=torch.int8)
+    w = torch.randint(-127, 128, (N, K), generator=g, device="cuda", dtype=torch.int8)
+    sizes = torch.tensor([3e38, 2.6e36, 1e33, 3e29, 1.9e19, 1.7e19, 1.0, 1e-12, 1e-30, 2e-38, 1e-41, 1.5e-45], device="cuda")
+    qs, ws = sizes[torch.arange(T, device="cuda") % 12], sizes.flip(0)[torch.arange(N, device="cuda") % 12]
+    y = abft.products.int8_matmul(q, qs, w, ws, dtype=dtype)
+    want = int_product(q, w) * qs.double()[:, None] * ws.double()
+    most = torch.finfo(dtype).max
+    inside, beyond = want.abs() < 0.99 * most, want.abs() > 1.01 * most
+    # the sum to 32 bits and two products with scales, the last one down to the smallest numbers: half a step each
+    tol = half_step(want, dtype) + want.abs() * (3 * 2.0 ** -24) * 1.01 + 2.0 ** -150
+    zero = torch.zeros((), dtype=torch.float64, device="cuda")
+    assert_near(torch.where(inside, y.double(), zero), torch.where(inside, want, zero), tol)
+    assert torch.equal(y[beyond].double(), torch.sign(want[beyond]) * math.inf)
+    assert inside.any() and beyond.any()
+
+
+def test_wide_range_rows_are_quantised_and_multiplied(abft):
+    """Rows near the largest numbers through a weight of small ones: the results are ordinary numbers."""
+    p, g = abft.products, gen(7)
+    for T in (2, 100):
+        x, w = (randn(g, T, 1000) * 1e37).bfloat16(), randn(g, 96, 1000) * 1e-35
+        wq, ws = p.quantize_rows(w)
+        q, s, e = p.quantize_rows(x, checksum=p.column_checksum(wq))
+        y, diff = p.int8_matmul(q, s, wq, ws, dtype=torch.float32, expect=e)
+        want = int_product(q, wq) * s.double()[:, None] * ws.double()
+        assert_near(y, want, half_step(want, torch.float32) + want.abs() * (3 * 2.0 ** -24) * 1.01)
+        assert (diff == 0).all() and want.abs().max() < 1e7
