@@ -1303,6 +1303,15 @@ bool extents(int T, int N, int K) {
     return T >= 0 && T <= kMost && N >= 1 && N <= kMost && K >= 1 && K <= kMost;
 }
 
+// Addresses of elements of `size` bytes; the kernels read and write them as such.
+bool lie_on(int size, std::initializer_list<const void*> pointers) {
+    for (const void* p : pointers)
+        if ((uintptr_t)p & (size - 1)) return false;
+    return true;
+}
+
+int size_of(int type) { return type == ABFT_TYPE_F32 ? 4 : 2; }
+
 bool holds(const void* work, size_t bytes, size_t needed) {
     return needed == 0 || (work && bytes >= needed && ((uintptr_t)work & 15) == 0);
 }
@@ -1653,6 +1662,8 @@ int abft_quantize_rows(const void* dX, int64_t ldx, int type, int T, int K, int8
     if (T == 0) return ABFT_OK;
     if (!dX || !dQ || !dScale || (dChecksum != nullptr) != (dExpect != nullptr))
         return bad("abft_quantize_rows: bad argument (missing pointer, or one of dChecksum and dExpect alone)");
+    if (!lie_on(size_of(type), {dX}) || !lie_on(4, {dScale, dChecksum}) || !lie_on(8, {dExpect}))
+        return bad("abft_quantize_rows: bad argument (a pointer not aligned to its elements)");
     const QuantArgs args{false, dX, ldx, T, K, dQ, ldq, dScale, dChecksum, dExpect};
     auto go = [&](auto tag) {
         return status(quantize<decltype(tag)>(args, (cudaStream_t)stream), "abft_quantize_rows");
@@ -1662,8 +1673,9 @@ int abft_quantize_rows(const void* dX, int64_t ldx, int type, int T, int K, int8
 }
 
 int abft_column_checksum(const int8_t* dW, int64_t ldw, int N, int K, int32_t* dChecksum, void* stream) {
-    if (!dW || !dChecksum || N < 1 || N > ABFT_INT8_MAX_ROWS || !extents(0, N, K) || ldw < K)
-        return bad("abft_column_checksum: bad argument (need pointers, 1 <= N <= 2^24, 1 <= K <= 2^30, ldw >= K)");
+    if (!dW || !dChecksum || N < 1 || N > ABFT_INT8_MAX_ROWS || !extents(0, N, K) || ldw < K || !lie_on(4, {dChecksum}))
+        return bad("abft_column_checksum: bad argument (need pointers, dChecksum aligned to its elements, 1 <= N <= 2^24, "
+                   "1 <= K <= 2^30, ldw >= K)");
     cudaStream_t s = (cudaStream_t)stream;
     const cudaError_t e = cudaMemsetAsync(dChecksum, 0, sizeof(int32_t) * K, s);
     if (e != cudaSuccess) return cuda_fail(e, "abft_column_checksum");
@@ -1691,6 +1703,8 @@ int abft_int8_matmul(const int8_t* dQ, int64_t ldq, const float* dQScale, const 
     if (T == 0) return ABFT_OK;
     if (!dQ || !dQScale || !dW || !dWScale || !dY || (dExpect != nullptr) != (dRowDiff != nullptr))
         return bad("abft_int8_matmul: bad argument (missing pointer, or one of dExpect and dRowDiff alone)");
+    if (!lie_on(size_of(type), {dY}) || !lie_on(4, {dQScale, dWScale}) || !lie_on(8, {dExpect, dRowDiff}))
+        return bad("abft_int8_matmul: bad argument (a pointer not aligned to its elements)");
     if (!holds(dWork, work_bytes, abft_int8_matmul_ws_bytes(dQ, ldq, dW, ldw, T, N, K)))
         return bad("abft_int8_matmul: workspace missing, too small or not 16-byte aligned");
     cudaStream_t s = (cudaStream_t)stream;
@@ -1737,6 +1751,8 @@ int abft_gated_ffn(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg
     if (T == 0) return ABFT_OK;
     if (!dX || !dWGate || !dWUp || !dH || (dG != nullptr) != (dU != nullptr))
         return bad("abft_gated_ffn: bad argument (missing pointer, or one of dG and dU alone)");
+    if (!lie_on(2, {dX, dWGate, dWUp, dH, dG, dU}))
+        return bad("abft_gated_ffn: bad argument (a pointer not aligned to its elements)");
     if (!holds(dWork, work_bytes, abft_gated_ffn_ws_bytes(dX, ldx, dWGate, ldwg, dWUp, ldwu, T, N, K)))
         return bad("abft_gated_ffn: workspace missing, too small or not 16-byte aligned");
     cudaStream_t s = (cudaStream_t)stream;
@@ -1778,6 +1794,8 @@ int abft_gated_ffn_backward(const void* dDH, int64_t ldd, const void* dX, int64_
         return bad("abft_gated_ffn_backward: bad argument (need 0 <= T <= 2^30, 1 <= N, K <= 2^30, pitches that hold "
                    "a row, a 16-bit element type and an activation)");
     if (!dDWGate || !dDWUp) return bad("abft_gated_ffn_backward: bad argument (missing pointer)");
+    if (!lie_on(2, {dDH, dX, dWGate, dWUp, dG, dU, dDX, dDWGate, dDWUp}))
+        return bad("abft_gated_ffn_backward: bad argument (a pointer not aligned to its elements)");
     cudaStream_t s = (cudaStream_t)stream;
     if (T == 0) {  // no token: the weights' gradients are empty sums
         cudaError_t e = cudaMemset2DAsync(dDWGate, lddwg * 2, 0, static_cast<size_t>(K) * 2, N, s);

@@ -255,8 +255,9 @@ int abft_sgemm(void* cublas_handle, const float* dA, int lda, const float* dB, i
  * streams are independent as long as their outputs and workspaces are. The
  * current device must be the stream's. Matrices are row-major with a pitch in
  * elements; a weight is N x K (one row per output channel). Element types are
- * ABFT_TYPE_*. T may be 0; T, N and K are at most ABFT_PRODUCT_MAX. Inputs and
- * outputs must not overlap.
+ * ABFT_TYPE_*. T may be 0; T, N and K are at most ABFT_PRODUCT_MAX. Pointers are
+ * aligned to their elements (others are refused). Inputs and outputs must not
+ * overlap.
  *
  * Workspaces: each *_ws_bytes function takes the inputs of its call and says
  * how many bytes of 16-byte aligned device memory that call needs as dWork
