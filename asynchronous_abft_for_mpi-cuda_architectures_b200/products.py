@@ -39,6 +39,9 @@ def _matrix(t, name, dtypes, rows=None, cols=None, device=None):
     pitch, step = t.stride()
     if step != 1 and c > 1:
         raise ValueError(f"{name} must be row-major (stride 1 along a row)")
+    # the imaginary part of a conjugate, whose memory holds the other sign; longer rows of it have a stride of 2
+    if c == 1 and t.is_neg():
+        raise ValueError(f"{name} is a view with a pending negation: resolve_neg() it first")
     if r <= 1:
         return (c + 15) & ~15  # one row has no pitch: any that keeps it aligned
     if pitch < c:
@@ -50,6 +53,8 @@ def _vector(t, name, dtype, n, device):
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype and t.shape == (n,)
             and (t.is_contiguous() or n <= 1)):
         raise ValueError(f"{name} must be a contiguous CUDA vector of {n} {str(dtype)[6:]}")
+    if n == 1 and t.is_neg():  # see _matrix; longer ones are not contiguous
+        raise ValueError(f"{name} is a view with a pending negation: resolve_neg() it first")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
 

@@ -164,3 +164,20 @@ def test_wide_range_rows_are_quantised_and_multiplied(abft):
         want = int_product(q, wq) * s.double()[:, None] * ws.double()
         assert_near(y, want, half_step(want, torch.float32) + want.abs() * (3 * 2.0 ** -24) * 1.01)
         assert (diff == 0).all() and want.abs().max() < 1e7
+
+
+# -------------------------------------------------------------- other views ---
+
+def test_views_with_a_pending_sign_are_refused(abft):
+    """The imaginary part of a conjugate holds the numbers with the other sign; resolved, it is a tensor like any other."""
+    p, g = abft.products, gen(8)
+    column = torch.randn(5, 1, dtype=torch.complex64, generator=g, device="cuda").conj().imag
+    one = torch.randn(1, dtype=torch.complex64, generator=g, device="cuda").conj().imag
+    assert column.is_neg() and one.is_neg()
+    q, s = p.quantize_rows(column.resolve_neg())
+    assert torch.equal(q.float(), 127 * column.resolve_neg().sign())
+    for bad in (lambda: p.quantize_rows(column), lambda: p.quantize_rows(column[:, 0].unsqueeze(1)),
+                lambda: p.quantize_rows(column[:1]), lambda: p.int8_matmul(q, s, q[:1], one),
+                lambda: p.int8_matmul(q[:1], one, q, s)):
+        with pytest.raises(ValueError):
+            bad()
