@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from conftest import PKG_NAME, ROOT
-from test_gpu_products import HALF, assert_near, block, gen, half_step, int_product, quantize_def, randn, same
+from test_gpu_products import HALF, assert_near, backward_def, block, gen, half_step, int_product, quantize_def, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -164,6 +164,85 @@ def test_wide_range_rows_are_quantised_and_multiplied(abft):
         want = int_product(q, wq) * s.double()[:, None] * ws.double()
         assert_near(y, want, half_step(want, torch.float32) + want.abs() * (3 * 2.0 ** -24) * 1.01)
         assert (diff == 0).all() and want.abs().max() < 1e7
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_quantize_every_value(dtype, abft):
+    """Every finite value of the type, under row maxima over its whole range, in rows held in registers and in wider ones."""
+    v = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype)
+    v = v[torch.isfinite(v)].cuda()
+    f = torch.finfo(dtype)
+    tops = [f.max, f.max * 0.7, f.smallest_normal, f.smallest_normal * f.eps, f.smallest_normal * f.eps * 5]
+    tops += [1.37 * 2.0 ** e for e in range(int(math.log2(f.smallest_normal)), int(math.log2(f.max)), 5)]
+    tops = torch.tensor(tops, dtype=torch.float64, device="cuda").to(dtype)
+    wide = torch.where(v.double().abs() <= tops.double()[:, None], v, torch.zeros_like(v))
+    short = torch.nn.functional.pad(wide, (0, -len(v) % 4095)).view(-1, 4095)
+    short = torch.cat([tops.repeat_interleave(short.shape[0] // len(tops))[:, None], short], 1)
+    for x in (wide, short, short[:, :200]):
+        q, scale = abft.products.quantize_rows(x)
+        want_q, want_s = quantize_def(x)
+        assert torch.equal(scale, want_s) and torch.equal(q, want_q)
+
+
+@pytest.mark.parametrize("T", [6, 200, 600])
+def test_float16_gradients_at_their_limit(T, abft):
+    """dgate is an operand of the products in the tensors' type: below 65504 the gradients are as ever; above, it is
+    infinite there, in the token's row of dx and the channel's row of dw_gate alone."""
+    dtype, N, K = torch.float16, 136, 72
+    r, x, wg, wu = block(T, T, N, K, dtype)
+    g, u, dh = (randn(r, T, N).to(dtype) for _ in range(3))
+    t, n = T // 2, 77
+    g[t, n], u[t, n] = 0.5, 2.0
+    slope = torch.sigmoid(torch.tensor(0.5)) * (1 + 0.5 * (1 - torch.sigmoid(torch.tensor(0.5))))
+    p = abft.products
+    dh[t, n] = 65000 / 2 / float(slope)
+    clean = p.gated_ffn_backward(dh, x, wg, wu, g, u)
+    # dgate = 65000 here, so that results pass the type's largest number where |x[t]| > 1.01: infinite by their own rounding
+    for grad, (want, tol) in zip(clean, backward_def(dh, x, wg, wu, g, u, "silu", dtype)):
+        most = torch.finfo(dtype).max
+        inside, beyond = want.abs() + tol < most, want.abs() - tol > most * (1 + torch.finfo(dtype).eps)
+        zero = torch.zeros((), dtype=torch.float64, device="cuda")
+        assert_near(torch.where(inside, grad.double(), zero), torch.where(inside, want, zero), tol)
+        assert torch.equal(grad[beyond].double(), torch.sign(want[beyond]) * math.inf)
+    dh[t, n] = 60000
+    dx, dwg, dwu = p.gated_ffn_backward(dh, x, wg, wu, g, u)
+    rows = torch.arange(T, device="cuda") != t
+    channels = torch.arange(N, device="cuda") != n
+    assert torch.equal(dx[rows], clean[0][rows]) and not dx[t].isfinite().any()
+    assert torch.equal(dwg[channels], clean[1][channels]) and not dwg[n].isfinite().any()
+    assert torch.equal(dwu[channels], clean[2][channels])
+
+
+def test_threads_at_once(abft):
+    """Four threads with streams of their own, calls of every size among one another: each gets its own bits."""
+    from concurrent.futures import ThreadPoolExecutor
+    p = abft.products
+    shapes = [(1, 300, 264), (40, 1000, 1032), (200, 264, 136), (1100, 1300, 96)]
+
+    def inputs(i):
+        T, N, K = shapes[i]
+        r, x, wg, wu = block(40 + i, T, N, K, torch.bfloat16)
+        return x, wg, wu, randn(r, T, N).bfloat16()
+
+    def run(x, wg, wu, dh):
+        h, g, u = p.gated_ffn(x, wg, wu, save=True)
+        w, ws = p.quantize_rows(wg)
+        q, s, e = p.quantize_rows(x, checksum=p.column_checksum(w))
+        return (h, *p.gated_ffn_backward(dh, x, wg, wu, g, u), *p.int8_matmul(q, s, w, ws, expect=e))
+    sets = [inputs(i) for i in range(4)]
+    wants = [run(*s) for s in sets]
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                got = run(*sets[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, wants[i])):
+                    return False
+        return True
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(work, range(4)))
 
 
 # -------------------------------------------------------------- other views ---
