@@ -49,8 +49,10 @@ constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 // The normal distribution function. With z = |g| / sqrt2 and t = 1 / (1 + 0.4 z) its
 // tail is erfc(z) / 2 = t e^(f(t) - z^2) / 2, f(t) = ln(e^(z^2) erfc(z) / t); f is smooth
 // on (0, 1], and a polynomial of degree 8 fitted to it (least squares at 4000
-// Chebyshev nodes of 0 <= z <= 14, 64 bits) is off by 1e-7; evaluated in 32 bits the
-// tail is off by 4.2e-7 relative, plus what the exponential loses of its argument.
+// Chebyshev nodes of 0 <= z <= 14, 64 bits) is off by 1.3e-7 with its coefficients as
+// they stand; evaluated in 32 bits the tail is off by 4.4e-7 relative up to |g| = 1,
+// 1.5e-6 up to 4 and 1.5e-5 up to 13 (the roundings of z and of the exponent, which grow
+// with it), plus what the exponential loses of its argument.
 // No branch and 18 instructions, where erfcf cost 3 to 4 us of results that are not
 // hidden behind products (1000 x 1536 x 1024 block: 13.5 us, 11.5 so).
 __device__ __forceinline__ float normal(float g) {
@@ -446,7 +448,13 @@ __global__ void __launch_bounds__(ROW < 128 ? 128 : ROW, 1024 / (ROW < 128 ? 128
 }
 
 // Column sums of an 8-bit weight: blocks of `rows` rows, their sums added as
-// integers (the order does not matter). WIDE: 4 columns per load.
+// integers (the order does not matter). WIDE: 4 columns per load. A weight's checksum
+// is taken once, when it is loaded; launched plainly, behind the memset of its sums.
+// Bound by reading w where it is wide (131072 x 8192: 203 us, 81 % of the copy rate),
+// else by a block's loads one after the other. Rows a block: 256 are best or as good
+// for large weights (131072 x 8192: 240 us with 64, 201 with 128, 203 with 256, 210 with
+// 1024; 8192 x 28672: 55 / 55 / 57 / 158); small ones would take fewer (4096 x 4096: 19
+// / 25 / 43 / 154).
 template <bool WIDE>
 __global__ void __launch_bounds__(256) k_column_checksum(const int8_t* __restrict__ w, int64_t ldw, int N, int K,
                                                          int rows, int32_t* __restrict__ checksum) {
@@ -588,7 +596,8 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, int limi
 // Tile order: groups of 16 tile rows, columns inside a group, so that the CTAs
 // at work at one time read few operand rows (L2 hits). 8192 x 16384 x 4096 block:
 // 1477 us with groups of 8, 1469 of 16, 1481 of 24; 8-bit product of 16384 x 16384 x
-// 4096: 732 / 717 / 717. The gradients sum over a long axis, along which all CTAs
+// 4096: 732 / 717 / 717 (all three sides in runs of the same length; that product now
+// takes 690 us in runs of 20 after a pause and 780 once the power cap has settled). The gradients sum over a long axis, along which all CTAs
 // move together and nothing stays in L2, so there the two operands' shares should
 // be alike: 3455 us with groups of 4, 3385 of 6, 3484 of 8, 3470 of 16.
 template <int MODE>
@@ -1203,8 +1212,8 @@ __global__ void __launch_bounds__(256, 2) k_few(const FewArgs a) {
 
 // What the rows' sums are added to. A kernel that starts beside the one before it
 // rather than a memset, which would end that: one quantised and verified token,
-// 16384 x 4096, replayed from a graph: 12.9 us against 16.1 (called eagerly, where
-// the host's 27 us are the bound, the memset saves 1.5 us).
+// 16384 x 4096, replayed from a graph on one weight: 12.4 us, 3.2 us less than with the
+// memset (called eagerly, where the host's 27 us are the bound, the memset saves 1.5 us).
 __global__ void __launch_bounds__(256) k_negate(const int64_t* __restrict__ in, int64_t* __restrict__ out, int n) {
     tensor::wait_for_stream();
     tensor::let_next_start();
@@ -1245,7 +1254,12 @@ __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
 }
 
 // dgate = dh u act'(g), dup = dh act(g). Bound by its five matrices; 8 elements
-// per thread where every row is 16-byte aligned (VEC).
+// per thread where every row is 16-byte aligned (VEC). Both are rounded once to the
+// tensors' type: the matrix instructions that take them as operands have 16 bits, and
+// it keeps the bytes that the two products read at half. A gradient is off by 2.35e-3
+// of its size (bfloat16) instead of the 1.66e-3 of its own rounding, by 2.9e-4 instead
+// of 2.1e-4 (float16). In float16 a dgate or dup above 65504 is infinite, as it is in
+// any program that keeps it in that type, in one row of dx and one channel of a weight.
 struct GradArgs {
     const void *dh, *g, *u;
     int64_t ldd, ldg, ldu;
@@ -1405,7 +1419,9 @@ int sm_count() {
 }
 
 // Threads per row and pieces held by each: the smallest that hold a row of K;
-// a warp alone needs no barrier.
+// a warp alone needs no barrier. Rows above 16384 do not fit a block's registers and
+// are read twice: 4096 rows of 28672 bfloat16 take 113 us (153 with a checksum, whose
+// 64-bit multiply-adds any K allows) where as many bytes in rows of 16384 take 62 (77).
 template <typename T>
 cudaError_t quantize(QuantArgs a, cudaStream_t s) {
     a.aligned = ((uintptr_t)a.x & 15) == 0 && (a.T == 1 || (a.ldx * (int64_t)sizeof(T) & 15) == 0) &&
@@ -1504,7 +1520,9 @@ int launch_product(const Operand (&a)[2], const Operand (&b)[2], ProductArgs arg
 // Whether k_few takes a product of T tokens with `bytes` of weights: always up to
 // 16; up to 32 while the weights are small, since past that its own work shows
 // (block of 16384 x 4096, 32 tokens: 65 us, 48 tokens by k_product 49 us; block of
-// 1024 x 4096: 7.8 against 10.2 us).
+// 1024 x 4096: 7.8 against 10.2 us). Operands off 16 bytes are copied before either
+// kernel, at the same cost (block of 16384 x 4097: 145 us for one token, 153 for 13,
+// by k_product 158 for 48), so the rule is theirs too.
 bool few_tokens(int T, int64_t bytes) { return T <= 16 || (T <= 32 && bytes <= 32 << 20); }
 
 template <bool GATE, typename E, typename O, int ACT = 0>

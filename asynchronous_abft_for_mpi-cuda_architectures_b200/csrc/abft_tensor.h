@@ -19,9 +19,10 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
-// Programmatic launch: every kernel of the products first waits until the work
-// before it in the stream is complete and visible, then lets the next one start
-// up beside it. What a kernel does before the wait touches no global memory.
+// Programmatic launch: every kernel of the products but the column checksum (which is
+// launched plainly) first waits until the work before it in the stream is complete and
+// visible, then lets the next one start up beside it. What a kernel does before the
+// wait touches no global memory.
 __device__ __forceinline__ void wait_for_stream() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -169,7 +169,9 @@ def int8_matmul(q, q_scale, w, w_scale, dtype=torch.bfloat16, expect=None, strea
     expect (from quantize_rows) verifies the product while it is computed:
     returns (y, rowdiff) with rowdiff[t] = sum_n sum_k q[t, k] * w[n, k] -
     expect[t] in exact integers, 0 for every sound row. A bit that flipped in q
-    or w since they were encoded, or in a sum, leaves a difference.
+    or w since they were encoded, or in a sum, leaves a difference in the rows it
+    reached, unless its effects on a row's sum cancel (a flip in q[t, k] where the
+    weight's column k sums to 0); the scaling after the sums is not covered.
     """
     ldq = _matrix(q, "q", (torch.int8,))
     T, K = q.shape
@@ -245,8 +247,9 @@ def gated_ffn_backward(dh, x, w_gate, w_up, g, u, activation="silu", stream=None
     """Gradients (dx, dw_gate, dw_up) of gated_ffn from dh (T x N) and the kept g, u.
 
     dgate = dh * u * act'(g) and dup = dh * act(g) are rounded to the tensors'
-    type (they are operands of the products); sums are in 32 bits and each
-    gradient is rounded once.
+    type (they are operands of the products): in float16 one above 65504 is
+    infinite, and with it its token's row of dx and its channel's row of the
+    weight's gradient. Sums are in 32 bits and each gradient is rounded once.
     """
     ldx, ldwg, ldwu, T, N, K = _block(x, w_gate, w_up)
     act = _activation(activation)

@@ -322,7 +322,8 @@ int abft_gated_ffn(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg
                    void* dU, int64_t ldu, void* dWork, size_t work_bytes, void* stream);
 
 /* Its gradients from dh (T x N) and the kept g, u:
- *   dgate = dh * u * act'(g), dup = dh * act(g)   (rounded to the type: operands of the products)
+ *   dgate = dh * u * act'(g), dup = dh * act(g)   (rounded to the type: operands of the products;
+ *                                                  above 65504 infinite in float16)
  *   dx = dgate Wgate + dup Wup (T x K), dWgate = dgate^T x, dWup = dup^T x (N x K)
  * Sums in 32 bits, each gradient rounded once; they are written, not added. */
 size_t abft_gated_ffn_backward_ws_bytes(const void* dX, int64_t ldx, const void* dWGate, int64_t ldwg,
