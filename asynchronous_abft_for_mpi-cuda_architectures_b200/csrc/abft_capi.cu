@@ -20,6 +20,7 @@ static thread_local std::string g_last_error;
 void set_error(const std::string& msg) { g_last_error = msg; }
 
 int cuda_fail(cudaError_t e, const char* what) {
+    (void)cudaGetLastError();  // told here: the next launch's check must not find it again
     set_error(std::string(what) + ": " + cudaGetErrorString(e));
     return ABFT_ERR_CUDA;
 }

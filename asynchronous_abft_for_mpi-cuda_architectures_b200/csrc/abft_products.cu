@@ -1438,7 +1438,10 @@ cudaError_t quantize(QuantArgs a, cudaStream_t s) {
         int64_t blocks = cdiv(a.T, kBlock / kRow);
         if (blocks > sm_count()) {  // as many as are resident at a time, each with the same number of rows
             int resident = 1;
-            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kBlock, smem) != cudaSuccess) resident = 1;
+            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kBlock, smem) != cudaSuccess) {
+                (void)cudaGetLastError();
+                resident = 1;
+            }
             blocks = std::min<int64_t>(blocks, (int64_t)sm_count() * std::max(resident, 1));
         }
         if (result == cudaSuccess) result = launch_next(kernel, dim3((unsigned)blocks), kBlock, smem, s, a);

@@ -129,6 +129,22 @@ def test_a_thread_is_told_of_a_fault_that_another_has_seen(abft):
         assert not told() and not other.submit(told).result()
 
 
+# --------------------------------------------------- after a call that failed ---
+
+def test_a_refused_call_does_not_fail_the_next(abft):
+    """An error that the CUDA runtime answers (a workspace larger than the GPU) is told once, by the call it belongs to."""
+    import ctypes
+    p, lib = abft.products, abft.lib
+    w = torch.randint(-128, 128, (40, 64), generator=gen(2), device="cuda", dtype=torch.int8)
+    want = p.column_checksum(w)
+    most = 1 << 30
+    one, zero, ws = (ctypes.c_int * 1)(most), (ctypes.c_int * 1)(0), ctypes.c_void_p()
+    assert lib.abft_ws_bytes(most, most, most, 1, one, most) > torch.cuda.get_device_properties(0).total_memory
+    assert lib.abft_ws_create(most, most, most, 1, one, zero, most, None, 0, ctypes.byref(ws)) == -2
+    assert torch.equal(p.column_checksum(w), want)
+    p.check_waits()
+
+
 # ------------------------------------------------------ the types' ranges ---
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
