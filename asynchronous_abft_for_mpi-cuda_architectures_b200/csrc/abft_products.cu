@@ -571,7 +571,7 @@ struct RowScale {
     float scale, back;
 
     explicit __device__ __forceinline__ RowScale(float s)
-        : scale(s >= 0x1p64f ? s * 0x1p-32f : s), back(s >= 0x1p64f ? 0x1p32f : 1.0f) {}
+        : scale(fabsf(s) >= 0x1p64f ? s * 0x1p-32f : s), back(fabsf(s) >= 0x1p64f ? 0x1p32f : 1.0f) {}
     __device__ __forceinline__ float times(int sum, float column) const {
         return static_cast<float>(sum) * scale * column * back;
     }

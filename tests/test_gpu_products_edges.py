@@ -169,6 +169,19 @@ def test_scales_over_the_whole_range(T, N, K, dtype, abft):
     assert inside.any() and beyond.any()
 
 
+@pytest.mark.parametrize("T", [3, 40, 200])
+def test_scales_of_either_sign(T, abft):
+    """A caller's own scales may be negative."""
+    g = gen(T)
+    q = torch.randint(-127, 128, (T, 2000), generator=g, device="cuda", dtype=torch.int8)
+    w = torch.randint(-127, 128, (70, 2000), generator=g, device="cuda", dtype=torch.int8)
+    sign = 1 - 2 * (torch.arange(200, device="cuda") % 2)
+    qs, ws = 2e37 * sign[:T], 1e-33 * sign[:70]
+    want = int_product(q, w) * qs.double()[:, None] * ws.double()
+    y = abft.products.int8_matmul(q, qs, w, ws, dtype=torch.float32)
+    assert_near(y, want, half_step(want, torch.float32) + want.abs() * (3 * 2.0 ** -24) * 1.01)
+
+
 def test_wide_range_rows_are_quantised_and_multiplied(abft):
     """Rows near the largest numbers through a weight of small ones: the results are ordinary numbers."""
     p, g = abft.products, gen(7)
